@@ -90,7 +90,7 @@ def draw(rng):
     hq = min(64, hkv * rng.choice([1, 2, 3, 4, 4, 5, 7, 8, 16])) // hkv * hkv
     if op == "append":
         chunk = rng.choice([1, 1, _log(rng, 2, 700)])
-        cap = 8192 * 48 // (hq + 2 * hkv) // chunk
+        cap = 6600 * 48 // (hq + 2 * hkv) // chunk
         return {"op": op, "batch": _log(rng, 1, max(1, min(512, cap))), "chunk": chunk, "hq": hq,
                 "hkv": hkv, "rot": rng.choice([128, 128, 96, 64]), "norm": rng.random() < 0.4,
                 "block": block}
