@@ -90,6 +90,27 @@ void rope_kv(at::Tensor& qkv, const at::Tensor& positions, const c10::optional<a
 void sample_tokens(const at::Tensor& logits, const at::Tensor& temperature,
                    const at::Tensor& top_k, const at::Tensor& top_p, const at::Tensor& seeds,
                    at::Tensor& out_tokens, const c10::optional<at::Tensor>& out_logprob);
+void step_tables(const at::Tensor& ctx_lens, const at::Tensor& q_lens,
+                 const c10::optional<at::Tensor>& rows, at::Tensor& seq_tables,
+                 const at::Tensor& new_blocks, at::Tensor& block_tables, at::Tensor& seq_lens,
+                 at::Tensor& cu_q, at::Tensor& positions, at::Tensor& slots,
+                 at::Tensor& last_rows, at::Tensor& tile_seq, at::Tensor& tile_row0,
+                 at::Tensor& num_new, int64_t block_size, int64_t group, int64_t rows_per_tile,
+                 int64_t num_decode, at::Tensor& err);
+void rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& slots,
+                 const at::Tensor& cos_sin, at::Tensor& k_cache, at::Tensor& v_cache,
+                 at::Tensor& k_scale, at::Tensor& v_scale, at::Tensor& q_out, int64_t hq,
+                 int64_t hkv, const c10::optional<at::Tensor>& q_norm,
+                 const c10::optional<at::Tensor>& k_norm, int64_t norm_dim, double eps,
+                 at::Tensor& err);
+void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
+                         const at::Tensor& v_cache, const at::Tensor& k_scale,
+                         const at::Tensor& v_scale, at::Tensor& out,
+                         const at::Tensor& block_tables, const at::Tensor& seq_lens,
+                         const c10::optional<at::Tensor>& cu_q,
+                         const c10::optional<at::Tensor>& tile_seq,
+                         const c10::optional<at::Tensor>& tile_row0, int64_t group, double scale,
+                         bool decode, bool causal, at::Tensor& err);
 }  // namespace lb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -165,4 +186,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("q_norm") = py::none(), py::arg("k_norm") = py::none(), py::arg("norm_dim") = 0,
         py::arg("eps") = 1e-6);
   m.def("sample_tokens", &lb::sample_tokens, "greedy / top-k / top-p sampling");
+  m.def("step_tables", &lb::step_tables,
+        "block tables, slot map, positions and attention work list of a step");
+  m.def("rope_kv_fp8", &lb::rope_kv_fp8,
+        "RoPE + append to the 8-bit paged KV cache (one scale per block and KV head)");
+  m.def("paged_attention_fp8", &lb::paged_attention_fp8,
+        "paged attention over the 8-bit KV cache (decode / prefill)");
 }

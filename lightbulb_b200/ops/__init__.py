@@ -423,3 +423,10 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
         out[r] = sample_row_reference(logits[r], float(temperature[r]), int(top_k[r]),
                                       float(top_p[r]), int(seeds[r]))
     return out
+
+
+# ------------------------------------------------------------------------------------
+# 8-bit paged KV cache
+# ------------------------------------------------------------------------------------
+from .fp8_kv import (FP8_KV_DTYPE, StepTables, paged_attention_fp8,  # noqa: E402,F401
+                     rope_kv_fp8, step_tables)
