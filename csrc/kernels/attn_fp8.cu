@@ -9,7 +9,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 
-#include "common.cuh"
+#include "attn_fp8.cuh"
 
 namespace lb {
 
@@ -17,30 +17,6 @@ void check_fp8_cache(const char* op, const at::Tensor& k_cache, const at::Tensor
                      const at::Tensor& k_scale, const at::Tensor& v_scale);
 
 namespace fp8a {
-
-constexpr int D = 128;
-
-struct Args {
-  const bf16* q;
-  int64_t q_ld;
-  bf16* out;
-  int64_t out_ld;
-  const uint8_t* k_cache;
-  const uint8_t* v_cache;
-  const float* k_scale;
-  const float* v_scale;
-  const int* tables;
-  int64_t bt_stride;
-  int bt_width;
-  const int* seq_lens;
-  const int* cu_q;        // nullptr: token i is sequence i's only one
-  const int* tile_seq;
-  const int* tile_row0;
-  int hq, hkv, group, bs, num_blocks, num_seqs;
-  int causal;
-  float scale_log2;
-  int* err;
-};
 
 __device__ __forceinline__ void unpack4(uint32_t v, float (&o)[4]) {
   uint32_t lo, hi;
@@ -55,14 +31,15 @@ __device__ __forceinline__ void unpack4(uint32_t v, float (&o)[4]) {
   o[0] = x.x; o[1] = x.y; o[2] = y.x; o[3] = y.y;
 }
 
-__device__ void attend(const Args& a, int seq, int64_t tok, int head, int klim, int lane) {
+__device__ void attend(const Args& a, const uint8_t* k_cache, const uint8_t* v_cache, int seq, int64_t tok, int head, int klim, int lane) {
   const int kvh = head / a.group;
   const uint2 raw = *reinterpret_cast<const uint2*>(a.q + tok * a.q_ld + head * D + lane * 4);
   const float2 qx = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
   const float2 qy = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
   float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  klim = min(klim, a.bt_width * a.bs);
-  for (int b = 0; b * a.bs < klim; ++b) {
+  const int bs = 1 << a.log2_bs;
+  klim = min(klim, a.bt_width * bs);
+  for (int b = 0; b * bs < klim; ++b) {
     int blk = a.tables[seq * a.bt_stride + b];
     if (static_cast<unsigned>(blk) >= static_cast<unsigned>(a.num_blocks)) {
       if (lane == 0) record_error(a.err, kErrBounds);
@@ -70,11 +47,11 @@ __device__ void attend(const Args& a, int seq, int64_t tok, int head, int klim, 
     }
     const int64_t bh = static_cast<int64_t>(blk) * a.hkv + kvh;
     const float ks = a.k_scale[bh] * a.scale_log2, vs = a.v_scale[bh];
-    const int n = min(a.bs, klim - b * a.bs);
+    const int n = min(bs, klim - b * bs);
     for (int j = 0; j < n; ++j) {
       float k[4], v[4];
-      unpack4(*reinterpret_cast<const uint32_t*>(a.k_cache + (bh * a.bs + j) * D + lane * 4), k);
-      unpack4(*reinterpret_cast<const uint32_t*>(a.v_cache + (bh * a.bs + j) * D + lane * 4), v);
+      unpack4(*reinterpret_cast<const uint32_t*>(k_cache + ((bh << a.log2_bs) + j) * D + lane * 4), k);
+      unpack4(*reinterpret_cast<const uint32_t*>(v_cache + ((bh << a.log2_bs) + j) * D + lane * 4), v);
       const float s = warp_sum(qx.x * k[0] + qx.y * k[1] + qy.x * k[2] + qy.y * k[3]) * ks;
       const float mn = fmaxf(m, s);
       const float corr = mn == -INFINITY ? 1.f : exp2f(m - mn);
@@ -90,16 +67,7 @@ __device__ void attend(const Args& a, int seq, int64_t tok, int head, int klim, 
   *reinterpret_cast<uint2*>(a.out + tok * a.out_ld + head * D + lane * 4) = r;
 }
 
-__global__ void __launch_bounds__(128) decode_kernel(const Args a) {
-  pdl_trigger();
-  pdl_wait();
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (w >= static_cast<int64_t>(a.num_seqs) * a.hq) return;
-  const int seq = w / a.hq;
-  attend(a, seq, seq, w % a.hq, a.seq_lens[seq], threadIdx.x & 31);
-}
-
-__global__ void __launch_bounds__(256) prefill_kernel(const Args a) {
+__global__ void __launch_bounds__(256) prefill_kernel(const Args a, const uint8_t* k_cache, const uint8_t* v_cache) {
   pdl_trigger();
   pdl_wait();
   const int seq = a.tile_seq[blockIdx.x];
@@ -113,7 +81,7 @@ __global__ void __launch_bounds__(256) prefill_kernel(const Args a) {
   for (int r = row0 + (threadIdx.x >> 5); r < min(row0 + 256, n * a.group); r += 8) {
     const int tok = r / a.group, g = r % a.group;
     const int klim = a.causal ? max(0, min(len, len - n + tok + 1)) : len;
-    attend(a, seq, q0 + tok, blockIdx.y * a.group + g, klim, threadIdx.x & 31);
+    attend(a, k_cache, v_cache, seq, q0 + tok, blockIdx.y * a.group + g, klim, threadIdx.x & 31);
   }
 }
 
@@ -150,8 +118,6 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   a.q_ld = q.stride(0);
   a.out = reinterpret_cast<bf16*>(out.data_ptr());
   a.out_ld = out.stride(0);
-  a.k_cache = reinterpret_cast<const uint8_t*>(k_cache.data_ptr());
-  a.v_cache = reinterpret_cast<const uint8_t*>(v_cache.data_ptr());
   a.k_scale = k_scale.data_ptr<float>();
   a.v_scale = v_scale.data_ptr<float>();
   a.tables = block_tables.data_ptr<int>();
@@ -163,18 +129,23 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   a.hq = q.size(1);
   a.hkv = k_cache.size(1);
   a.group = group;
-  a.bs = k_cache.size(2);
+  a.log2_bs = k_cache.size(2) == 16 ? 4 : k_cache.size(2) == 32 ? 5 : 6;
   a.num_blocks = k_cache.size(0);
   a.num_seqs = B;
   a.causal = causal ? 1 : 0;
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   a.err = err.data_ptr<int>();
+  // a row of 128 codes is 64 two-byte elements to the tensor map
+  const uint64_t rows = k_cache.size(0) * k_cache.size(1) * k_cache.size(2);
+  const CUtensorMap tk =
+      make_tmap_bf16_2d(k_cache.data_ptr(), 64, rows, D, 64, SL, CU_TENSOR_MAP_SWIZZLE_128B);
+  const CUtensorMap tv =
+      make_tmap_bf16_2d(v_cache.data_ptr(), 64, rows, D, 64, SL, CU_TENSOR_MAP_SWIZZLE_128B);
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   if (decode) {
     TORCH_CHECK(q.size(0) >= B, op, ": one query token per sequence");
     if (B == 0) return;
-    C10_CUDA_CHECK(launch_k(decode_kernel, dim3((B * a.hq + 3) / 4), dim3(128), 0, st, nullptr,
-                            0, a));
+    fp8_decode(a, tk, tv, q, st);
     return;
   }
   TORCH_CHECK(cu_q.has_value() && tile_seq.has_value() && tile_row0.has_value(), op,
@@ -188,7 +159,8 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   a.tile_seq = tile_seq->data_ptr<int>();
   a.tile_row0 = tile_row0->data_ptr<int>();
   C10_CUDA_CHECK(launch_k(prefill_kernel, dim3(tile_seq->numel(), a.hkv), dim3(256), 0, st,
-                          nullptr, 0, a));
+                          nullptr, 0, a, reinterpret_cast<const uint8_t*>(k_cache.data_ptr()),
+                          reinterpret_cast<const uint8_t*>(v_cache.data_ptr())));
 }
 
 }  // namespace lb
