@@ -83,5 +83,7 @@ __device__ __forceinline__ int checked_block(const Args& a, int id) {
 // Launch on the current stream; the tensor maps view the caches as rows of 128 bytes.
 void fp8_decode(const fp8a::Args& a, const CUtensorMap& tk, const CUtensorMap& tv,
                 const at::Tensor& like, cudaStream_t st);
+void fp8_prefill(const fp8a::Args& a, const CUtensorMap& tk, const CUtensorMap& tv,
+                 cudaStream_t st);
 
 }  // namespace lb
