@@ -90,13 +90,11 @@ void rope_kv(at::Tensor& qkv, const at::Tensor& positions, const c10::optional<a
 void sample_tokens(const at::Tensor& logits, const at::Tensor& temperature,
                    const at::Tensor& top_k, const at::Tensor& top_p, const at::Tensor& seeds,
                    at::Tensor& out_tokens, const c10::optional<at::Tensor>& out_logprob);
-void step_tables(const at::Tensor& ctx_lens, const at::Tensor& q_lens,
-                 const c10::optional<at::Tensor>& rows, at::Tensor& seq_tables,
-                 const at::Tensor& new_blocks, at::Tensor& block_tables, at::Tensor& seq_lens,
-                 at::Tensor& cu_q, at::Tensor& positions, at::Tensor& slots,
-                 at::Tensor& last_rows, at::Tensor& tile_seq, at::Tensor& tile_row0,
-                 at::Tensor& num_new, int64_t block_size, int64_t group, int64_t rows_per_tile,
-                 int64_t num_decode, at::Tensor& err);
+std::vector<at::Tensor> step_tables(const at::Tensor& ctx_lens, const at::Tensor& q_lens,
+                                    const c10::optional<at::Tensor>& rows, at::Tensor& seq_tables,
+                                    const at::Tensor& new_blocks, int64_t num_tokens,
+                                    int64_t block_size, int64_t group, int64_t rows_per_tile,
+                                    int64_t num_decode, at::Tensor& err);
 void rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& slots,
                  const at::Tensor& cos_sin, at::Tensor& k_cache, at::Tensor& v_cache,
                  at::Tensor& k_scale, at::Tensor& v_scale, at::Tensor& q_out, int64_t hq,

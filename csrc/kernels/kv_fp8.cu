@@ -39,7 +39,7 @@ struct Args {
   float* v_scale;
   const bf16* q_norm;
   const bf16* k_norm;
-  float norm_dim, eps;
+  float inv_norm_dim, eps;
   int T, hq, hkv, bs, num_blocks;
   int* err;
 };
@@ -74,120 +74,346 @@ __device__ __forceinline__ int scale_exp(float amax) {
   const int k = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
   return min(MAX_EXP, max(MIN_EXP, k));
 }
+__device__ __forceinline__ float max_abs(float m, float a, float b) {
+  return fmaxf(m, fmaxf(fabsf(a), fabsf(b)));
+}
 __device__ __forceinline__ float exp2i(int k) { return __uint_as_float((k + 127) << 23); }
 
-// Row t's head at src, 4 elements per lane: optional RMSNorm, then the rotation.  Products and
-// sums are rounded one by one, as the formula's separate operations are.
-__device__ __forceinline__ void load_rotated(const Args& a, const bf16* src, int t, int lane,
-                                             const bf16* nw, bool rotate, float (&o)[4]) {
-  const uint2 raw = *reinterpret_cast<const uint2*>(src + lane * 4);
-  const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
-  const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
-  float v[4] = {x.x, x.y, y.x, y.y};
-  if (nw != nullptr) {
-    const float ss = warp_sum(v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3]);
-    const float inv = rsqrtf(ss / a.norm_dim + a.eps);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = __fmul_rn(__fmul_rn(v[i], inv), __bfloat162float(nw[lane * 4 + i]));
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = v[i];
-  if (!rotate) return;
+// Half a warp holds one head row.  A lane owns both partners of its rotations: four dims from d0 and
+// their partners from d1 = d0 + rot / 2, so nothing is exchanged between lanes; lanes past the
+// rotary width hold two runs of four dims that pass through.  The instructions per element bound
+// this kernel before HBM does, so the arithmetic runs on fp32 pairs (mul / add .f32x2).  Products
+// and sums are rounded one by one, as the formula's separate operations are.
+typedef uint64_t f2;
+__device__ __forceinline__ f2 pack2(float lo, float hi) {
+  f2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpack2(f2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f2 sub2(f2 a, f2 b) {
+  f2 d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f2 widen(uint32_t bf16_pair) {
+  return pack2(__uint_as_float(bf16_pair << 16), __uint_as_float(bf16_pair & 0xffff0000u));
+}
+
+struct Lane {
+  int d0, d1;      // first dim of the two runs of four
+  bool in;         // rotates
+};
+__device__ __forceinline__ Lane lane_of(const Args& a, int lane) {
+  Lane r;
+  const int hl = lane & 15, half = a.rot >> 1;
+  r.in = hl * 4 < half;
+  r.d0 = r.in ? hl * 4 : a.rot + 8 * (hl - (half >> 2));
+  r.d1 = r.in ? half + hl * 4 : r.d0 + 4;
+  return r;
+}
+__device__ __forceinline__ uint4 load_row(const bf16* p, const Lane& ro) {
+  const uint2 x = *reinterpret_cast<const uint2*>(p + ro.d0);
+  const uint2 y = *reinterpret_cast<const uint2*>(p + ro.d1);
+  return make_uint4(x.x, x.y, y.x, y.y);
+}
+__device__ __forceinline__ void widen4(const uint4& raw, f2 (&v)[4]) {
+  v[0] = widen(raw.x);
+  v[1] = widen(raw.y);
+  v[2] = widen(raw.z);
+  v[3] = widen(raw.w);
+}
+struct Turn {      // cos and sin of a lane's four rotations
+  f2 c[2] = {0, 0}, s[2] = {0, 0};
+};
+__device__ __forceinline__ void load_turn(const Args& a, const Lane& ro, int lane, int t, Turn& tu) {
   int pos = a.positions[t];
   if (static_cast<unsigned>(pos) >= static_cast<unsigned>(a.max_pos)) {
-    if (lane == 0) record_error(a.err, kErrBounds);
+    if ((lane & 15) == 0) record_error(a.err, kErrBounds);
     pos = 0;
   }
-  const int half = a.rot >> 1, e0 = lane * 4;
-  const bool rot = e0 < a.rot, first = e0 < half;
-  const int plane = !rot ? lane : (first ? lane + (half >> 2) : lane - (half >> 2));
-  float p[4];
+  if (ro.in) {
+    const float* p = a.cos_sin + static_cast<size_t>(pos) * a.rot + ro.d0;
+    const float4 c = *reinterpret_cast<const float4*>(p);
+    const float4 s = *reinterpret_cast<const float4*>(p + (a.rot >> 1));
+    tu.c[0] = pack2(c.x, c.y);
+    tu.c[1] = pack2(c.z, c.w);
+    tu.s[0] = pack2(s.x, s.y);
+    tu.s[1] = pack2(s.z, s.w);
+  }
+}
+// In place; both halves of the warp take part.
+__device__ __forceinline__ void norm_turn(const Args& a, const Lane& ro, const f2* w, const Turn& tu,
+                                          f2 (&v)[4]) {
+  if (w != nullptr) {
+    f2 q = mul2(v[0], v[0]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = __shfl_sync(0xffffffffu, v[i], plane);
-  if (rot) {
-    const float* cs = a.cos_sin + static_cast<size_t>(pos) * a.rot + (first ? e0 : e0 - half);
+    for (int i = 1; i < 4; ++i) q = fma2(v[i], v[i], q);
+    float lo, hi;
+    unpack2(q, lo, hi);
+    float ss = lo + hi;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float c = cs[i], s = cs[half + i];
-      o[i] = first ? __fsub_rn(__fmul_rn(v[i], c), __fmul_rn(p[i], s))
-                   : __fadd_rn(__fmul_rn(p[i], s), __fmul_rn(v[i], c));
+    for (int m = 1; m < 16; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+    const float inv = rsqrtf(ss * a.inv_norm_dim + a.eps);
+    const f2 inv2 = pack2(inv, inv);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = mul2(mul2(v[i], inv2), w[i]);
+  }
+  if (ro.in) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f2 x = v[i], y = v[i + 2];
+      v[i] = sub2(mul2(x, tu.c[i]), mul2(y, tu.s[i]));
+      v[i + 2] = add2(mul2(x, tu.s[i]), mul2(y, tu.c[i]));
+    }
+  }
+}
+__device__ __forceinline__ uint32_t bf16_pair(f2 v) {
+  float lo, hi;
+  unpack2(v, lo, hi);
+  return pack_bf16x2(lo, hi);
+}
+__device__ __forceinline__ uint32_t codes4(f2 a, f2 b, f2 inv) {
+  float x[4];
+  unpack2(mul2(a, inv), x[0], x[1]);
+  unpack2(mul2(b, inv), x[2], x[3]);
+  return e4m3x4(x[0], x[1], x[2], x[3]);
+}
+
+// ---- q: a warp takes two rows and HPW heads; the rows' cos and sin stay in registers ----
+constexpr int HPW = 4;
+__device__ __forceinline__ void rotate_q(const Args& a, int64_t w, int lane) {
+  const int groups = (a.hq + HPW - 1) / HPW;
+  const int t = static_cast<int>(w / groups) * 2 + (lane >> 4);
+  const int h0 = static_cast<int>(w % groups) * HPW;
+  const Lane ro = lane_of(a, lane);
+  const bool live = t < a.T;
+  const int n = live ? min(HPW, a.hq - h0) : 0;
+  const bf16* src = a.qkv + t * a.ld + h0 * D;
+  uint4 raw[HPW];
+#pragma unroll
+  for (int i = 0; i < HPW; ++i)
+    raw[i] = i < n ? load_row(src + i * D, ro) : make_uint4(0, 0, 0, 0);
+  Turn tu;
+  if (live) load_turn(a, ro, lane, t, tu);
+  f2 nw[4];
+  const bool norm = a.q_norm != nullptr;
+  if (norm) widen4(load_row(a.q_norm, ro), nw);
+  bf16* dst = a.q_out + t * a.q_ld + h0 * D;
+#pragma unroll
+  for (int i = 0; i < HPW; ++i) {
+    f2 v[4];
+    widen4(raw[i], v);
+    norm_turn(a, ro, norm ? nw : nullptr, tu, v);
+    if (i < n) {
+      *reinterpret_cast<uint2*>(dst + i * D + ro.d0) = make_uint2(bf16_pair(v[0]), bf16_pair(v[1]));
+      *reinterpret_cast<uint2*>(dst + i * D + ro.d1) = make_uint2(bf16_pair(v[2]), bf16_pair(v[3]));
     }
   }
 }
 
-__global__ void __launch_bounds__(THREADS) rope_kv_fp8_kernel(const Args a) {
-  pdl_trigger();
-  pdl_wait();
-  const int heads = a.hq + 2 * a.hkv;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * (THREADS / 32) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (w >= static_cast<int64_t>(a.T) * heads) return;      // warp-uniform
-  const int t = static_cast<int>(w / heads), h = static_cast<int>(w % heads);
-  if (h < a.hq) {
-    float o[4];
-    load_rotated(a, a.qkv + t * a.ld + h * D, t, lane, a.q_norm, true, o);
-    const uint2 out = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
-    *reinterpret_cast<uint2*>(a.q_out + t * a.q_ld + h * D + lane * 4) = out;
-    return;
-  }
-  // k or v head: the warp of the first row that goes to a block handles all of its rows
-  const int slot = a.slots[t];
-  if (slot < 0) return;
-  const int blk = slot / a.bs;
-  if (blk >= a.num_blocks) {
-    if (lane == 0) record_error(a.err, kErrBounds);
-    return;
-  }
-  for (int i = 0; i < a.bs - 1; i += 32) {
-    const int r = t - 1 - i - lane;
-    const int s = r >= 0 && i + lane < a.bs - 1 ? a.slots[r] : -1;
-    if (__any_sync(0xffffffffu, s >= 0 && s / a.bs == blk)) return;
-  }
-  const bool is_v = h >= a.hq + a.hkv;
-  const int kh = is_v ? h - a.hq - a.hkv : h - a.hq;
-  const bf16* nw = is_v ? nullptr : a.k_norm;
-  const int end = min(a.T, t + a.bs);
-  float amax = 0.f;
-  for (int r = t; r < end; ++r) {
-    const int s = a.slots[r];
-    if (s < 0 || s / a.bs != blk) continue;
-    float o[4];
-    load_rotated(a, a.qkv + r * a.ld + h * D, r, lane, nw, !is_v, o);
+// ---- k, v: NW warps take the blocks that are entered in `win` consecutive rows, HPK heads ----
+//
+// The slots of the window and of BS rows on both sides sit in the lanes (row base + 32 k + lane in
+// sl[k]); a ballot per block gives its rows.  A block belongs to the window that holds its first
+// row.  Rows are rotated into registers four at a time per warp (two per step, half a warp each):
+// while a block's rows fit the NW warps they are read once, otherwise twice (maximum, then codes).
+constexpr int HPK = 2;
+template <int BS, int NW>
+__device__ __forceinline__ void append_kv(const Args& a, int64_t w, int win, int warp, int lane,
+                                          float (*s_max)[HPK]) {
+  constexpr int NR = (2 * BS + 16 + 31) / 32;
+  const int groups = (a.hkv + HPK - 1) / HPK;
+  const int w0 = static_cast<int>(w / (2 * groups)) * win, gi = static_cast<int>(w % (2 * groups));
+  const bool is_v = gi >= groups;
+  const int kh0 = (is_v ? gi - groups : gi) * HPK;
+  const int base = w0 - BS;
+  int sl[NR];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(o[i]));
+  for (int k = 0; k < NR; ++k) {
+    const int r = base + 32 * k + lane;
+    sl[k] = r >= 0 && r < a.T ? a.slots[r] : -1;
   }
-  amax = warp_max(amax);
-  float* sp = (is_v ? a.v_scale : a.k_scale) + static_cast<int64_t>(blk) * a.hkv + kh;
-  uint8_t* base = (is_v ? a.v_cache : a.k_cache) +
-                  (static_cast<int64_t>(blk) * a.hkv + kh) * a.bs * D;
-  const int first = slot - blk * a.bs;
-  float scale = exp2i(scale_exp(amax));
-  if (first > 0) {
-    const float old = *sp;
-    if (old >= scale) {
-      scale = old;
-    } else {
-      const float ratio = old / scale;
-      for (int r = 0; r < first; ++r) {
-        uint32_t* p = reinterpret_cast<uint32_t*>(base + r * D) + lane;
-        float o[4];
-        e4m3x4_to_f32(*p, o);
-        *p = e4m3x4(o[0] * ratio, o[1] * ratio, o[2] * ratio, o[3] * ratio);
+  const Lane ro = lane_of(a, lane);
+  const bool norm = !is_v && a.k_norm != nullptr;
+  f2 nw[4];
+  if (norm) widen4(load_row(a.k_norm, ro), nw);
+  // rows of the window that have a slot
+  const int i0 = BS, i1 = BS + min(win, a.T - w0);
+  uint32_t todo[NR];
+#pragma unroll
+  for (int k = 0; k < NR; ++k)
+    todo[k] = __ballot_sync(0xffffffffu, sl[k] >= 0 && 32 * k + lane >= i0 && 32 * k + lane < i1);
+  const bf16* head =
+      a.qkv + static_cast<int64_t>(a.hq + (is_v ? a.hkv : 0) + kh0) * D;
+  float* scales = is_v ? a.v_scale : a.k_scale;
+  uint8_t* cache = is_v ? a.v_cache : a.k_cache;
+  while (true) {
+    int first = -1, slot = 0;
+#pragma unroll
+    for (int k = NR - 1; k >= 0; --k)
+      if (todo[k]) {
+        first = 32 * k + __ffs(todo[k]) - 1;
+        slot = __shfl_sync(0xffffffffu, sl[k], first & 31);
       }
+    if (first < 0) break;
+    const int blk = slot / BS;
+    bool earlier = false;
+    int last = first;
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+      const int i = 32 * k + lane;
+      const bool same = sl[k] >= 0 && sl[k] / BS == blk;
+      earlier |= __any_sync(0xffffffffu, same && i < first && i > first - BS) != 0;
+      const uint32_t mem = __ballot_sync(0xffffffffu, same && i >= first && i < first + BS);
+      todo[k] &= ~mem;
+      if (mem) last = 32 * k + 31 - __clz(mem);
+    }
+    if (earlier) continue;                          // another window's block
+    if (blk >= a.num_blocks) {
+      if (lane == 0) record_error(a.err, kErrBounds);
+      continue;
+    }
+    const int row_a = base + first, row_b = base + last;
+    const int chunks = (row_b - row_a + 4 * NW) / (4 * NW);
+    const int64_t bh = static_cast<int64_t>(blk) * a.hkv + kh0;
+    float old[HPK];
+#pragma unroll
+    for (int h = 0; h < HPK; ++h) old[h] = kh0 + h < a.hkv ? scales[bh + h] : 0.f;
+    f2 v[2][HPK][4];
+    int off[2];                                     // the row's place in the block, -1: none
+    auto load = [&](int c) {
+      uint4 raw[2][HPK];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = row_a + (c * NW + warp) * 4 + 2 * i + (lane >> 4);
+        const int x = row <= row_b ? a.slots[row] : -1;
+        off[i] = x >= 0 && x / BS == blk ? x - blk * BS : -1;
+#pragma unroll
+        for (int h = 0; h < HPK; ++h)
+          raw[i][h] = off[i] >= 0 && kh0 + h < a.hkv
+                          ? load_row(head + row * a.ld + h * D, ro)
+                          : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int h = 0; h < HPK; ++h) widen4(raw[i][h], v[i][h]);
+        if (!is_v) {
+          const int row = row_a + (c * NW + warp) * 4 + 2 * i + (lane >> 4);
+          Turn tu;
+          if (off[i] >= 0) load_turn(a, ro, lane, row, tu);
+#pragma unroll
+          for (int h = 0; h < HPK; ++h) norm_turn(a, ro, norm ? nw : nullptr, tu, v[i][h]);
+        }
+      }
+    };
+    float amax[HPK];
+#pragma unroll
+    for (int h = 0; h < HPK; ++h) amax[h] = 0.f;
+    for (int c = 0; c < chunks; ++c) {
+      load(c);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < HPK; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float lo, hi;
+            unpack2(v[i][h][e], lo, hi);
+            amax[h] = max_abs(amax[h], lo, hi);
+          }
+    }
+#pragma unroll
+    for (int h = 0; h < HPK; ++h) amax[h] = warp_max(amax[h]);
+    if (NW > 1) {
+      __syncthreads();                              // s_max of the previous block has been read
+      if (lane == 0) {
+#pragma unroll
+        for (int h = 0; h < HPK; ++h) s_max[warp][h] = amax[h];
+      }
+      __syncthreads();                              // and every warp has read the old scales
+#pragma unroll
+      for (int h = 0; h < HPK; ++h)
+#pragma unroll
+        for (int k = 0; k < NW; ++k) amax[h] = fmaxf(amax[h], s_max[k][h]);
+    }
+    const int entry = slot - blk * BS;
+    float inv[HPK];
+#pragma unroll
+    for (int h = 0; h < HPK; ++h) {
+      if (kh0 + h >= a.hkv) continue;
+      float scale = exp2i(scale_exp(amax[h]));
+      if (entry > 0) {
+        if (old[h] >= scale) {
+          scale = old[h];
+        } else {
+          const float ratio = old[h] / scale;
+          for (int r = warp * 2 + (lane >> 4); r < entry; r += 2 * NW) {
+            uint8_t* p = cache + ((bh + h) * BS + r) * D;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t* x = reinterpret_cast<uint32_t*>(p + (e ? ro.d1 : ro.d0));
+              float f[4];
+              e4m3x4_to_f32(*x, f);
+              *x = e4m3x4(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+            }
+          }
+        }
+      }
+      inv[h] = 1.f / scale;
+      __syncwarp();                                 // NW == 1: every lane has read the old scale
+      if (warp == 0 && lane == 0) scales[bh + h] = scale;
+    }
+    for (int c = chunks - 1; c >= 0; --c) {
+      if (c != chunks - 1) load(c);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < HPK; ++h)
+          if (off[i] >= 0 && kh0 + h < a.hkv) {
+            const f2 s = pack2(inv[h], inv[h]);
+            uint8_t* p = cache + ((bh + h) * BS + off[i]) * D;
+            *reinterpret_cast<uint32_t*>(p + ro.d0) = codes4(v[i][h][0], v[i][h][1], s);
+            *reinterpret_cast<uint32_t*>(p + ro.d1) = codes4(v[i][h][2], v[i][h][3], s);
+          }
     }
   }
-  const float inv = 1.f / scale;
-  for (int r = t; r < end; ++r) {
-    const int s = a.slots[r];
-    if (s < 0 || s / a.bs != blk) continue;
-    float o[4];
-    load_rotated(a, a.qkv + r * a.ld + h * D, r, lane, nw, !is_v, o);
-    *(reinterpret_cast<uint32_t*>(base + (s - blk * a.bs) * D) + lane) =
-        e4m3x4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+}
+
+template <int BS, int NW>
+__global__ void __launch_bounds__(THREADS, 5) rope_kv_fp8_kernel(const Args a, int win,
+                                                              int kv_ctas) {
+  __shared__ float s_max[THREADS / 32][HPK];
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int WPC = THREADS / 32;
+  if (static_cast<int>(blockIdx.x) < kv_ctas) {
+    const int64_t items = static_cast<int64_t>((a.T + win - 1) / win) * 2 * ((a.hkv + HPK - 1) / HPK);
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * (WPC / NW) + warp / NW;
+    if (w < items) append_kv<BS, NW>(a, w, win, warp % NW, lane, s_max);
+  } else {
+    const int64_t w = static_cast<int64_t>(blockIdx.x - kv_ctas) * WPC + warp;
+    if (w < static_cast<int64_t>((a.T + 1) / 2) * ((a.hq + HPW - 1) / HPW)) rotate_q(a, w, lane);
   }
-  __syncwarp();
-  if (lane == 0) *sp = scale;
 }
 
 }  // namespace kq
@@ -267,7 +493,7 @@ void rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const at::T
   a.v_cache = reinterpret_cast<uint8_t*>(v_cache.data_ptr());
   a.k_scale = k_scale.data_ptr<float>();
   a.v_scale = v_scale.data_ptr<float>();
-  a.norm_dim = norm_dim > 0 ? static_cast<float>(norm_dim) : static_cast<float>(R);
+  a.inv_norm_dim = 1.f / (norm_dim > 0 ? static_cast<float>(norm_dim) : static_cast<float>(R));
   a.eps = static_cast<float>(eps);
   a.T = T;
   a.hq = hq;
@@ -275,9 +501,22 @@ void rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const at::T
   a.bs = k_cache.size(2);
   a.num_blocks = k_cache.size(0);
   a.err = err.data_ptr<int>();
-  const int64_t warps = T * (hq + 2 * hkv);
-  C10_CUDA_CHECK(launch_k(rope_kv_fp8_kernel, dim3((warps + THREADS / 32 - 1) / (THREADS / 32)),
-                          dim3(THREADS), 0, at::cuda::getCurrentCUDAStream(), nullptr, 0, a));
+  // A warp per row (and head pair) while that leaves the GPU room: a decode batch, every row its own
+  // block.  Beyond that the rows are mostly chunks of prompts: four warps share a window of 16 rows,
+  // which holds about one block, and read it once.
+  constexpr int WPC = THREADS / 32;
+  const int64_t pairs = 2 * ((hkv + HPK - 1) / HPK);
+  const bool few = T * pairs <= 148 * 32;
+  const int win = few ? 1 : 16;
+  const int64_t kv = few ? (T * pairs + WPC - 1) / WPC : (T + 15) / 16 * pairs;
+  const int64_t qw = ((T + 1) / 2 * ((hq + HPW - 1) / HPW) + WPC - 1) / WPC;
+  TORCH_CHECK(kv + qw < (int64_t(1) << 31), "rope_kv_fp8: too many rows");
+  auto kernel = a.bs == 16   ? (few ? rope_kv_fp8_kernel<16, 1> : rope_kv_fp8_kernel<16, 4>)
+                : a.bs == 32 ? (few ? rope_kv_fp8_kernel<32, 1> : rope_kv_fp8_kernel<32, 4>)
+                             : (few ? rope_kv_fp8_kernel<64, 1> : rope_kv_fp8_kernel<64, 4>);
+  C10_CUDA_CHECK(launch_k(kernel, dim3(kv + qw), dim3(THREADS), 0,
+                          at::cuda::getCurrentCUDAStream(), nullptr, 0, a, win,
+                          static_cast<int>(kv)));
 }
 
 }  // namespace lb

@@ -16,6 +16,7 @@
 // tokens, table entries and tiles, finding the owner of an item by bisection in shared memory.
 // A slot in a block that this step adds is taken from new_blocks, never from the table that
 // another CTA is writing.
+#include <ATen/Functions.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -27,6 +28,7 @@ namespace st {
 
 constexpr int THREADS = 256;
 constexpr int MAX_B = 4096;
+constexpr int SEG = 128;          // table entries per warp step
 
 struct Args {
   const int* ctx;
@@ -161,25 +163,27 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const Args a) {
     a.positions[i] = pos;
     a.slots[i] = slot;
   }
-  // the batch's tables, one warp per request; new entries also go to the resident table
-  for (int b = gt >> 5; b < a.B; b += nthreads >> 5) {
+  // the batch's tables, SEG entries of one request per warp; new entries also go to the resident
+  // table
+  const int segs = (a.W + SEG - 1) / SEG;
+  for (int i = gt >> 5; i < a.B * segs; i += nthreads >> 5) {
+    const int b = i / segs, j0 = (i - b * segs) * SEG + lane;
     const int n = sq[b + 1] - sq[b];
     const int have = (sc[b] + bs - 1) >> a.log2_bs, need = (sc[b] + n + bs - 1) >> a.log2_bs;
     const int row = a.rows != nullptr ? a.rows[b] : b;
     int* src = a.seq_tables + (need > 0 ? row * a.tab_stride : 0);
     int* dst = a.block_tables + static_cast<int64_t>(b) * a.W;
-    for (int j = lane; j < a.W; j += 32) {
-      int id = 0;
-      if (j < have) {
-        id = src[j];
-      } else if (j < need) {
-        const int f = sn[b] + j - have;
-        if (f < a.F) {
-          id = a.new_blocks[f];
-          src[j] = id;
-        }
-      }
-      dst[j] = id;
+    int id[SEG / 32];
+#pragma unroll
+    for (int k = 0; k < SEG / 32; ++k) {
+      const int j = j0 + 32 * k, f = sn[b] + j - have;
+      id[k] = j < have ? src[j] : j < need && f < a.F ? a.new_blocks[f] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < SEG / 32; ++k) {
+      const int j = j0 + 32 * k;
+      if (j < a.W) dst[j] = id[k];
+      if (j >= have && j < need && sn[b] + j - have < a.F) src[j] = id[k];
     }
   }
   for (int i = gt; i < a.num_tiles; i += nthreads) {
@@ -196,40 +200,55 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const Args a) {
 
 }  // namespace st
 
-void step_tables(const at::Tensor& ctx_lens, const at::Tensor& q_lens,
-                 const c10::optional<at::Tensor>& rows, at::Tensor& seq_tables,
-                 const at::Tensor& new_blocks, at::Tensor& block_tables, at::Tensor& seq_lens,
-                 at::Tensor& cu_q, at::Tensor& positions, at::Tensor& slots,
-                 at::Tensor& last_rows, at::Tensor& tile_seq, at::Tensor& tile_row0,
-                 at::Tensor& num_new, int64_t block_size, int64_t group, int64_t rows_per_tile,
-                 int64_t num_decode, at::Tensor& err) {
+// Contiguous int32 view of `n` elements (or [r, n / r]) of a buffer.
+static at::Tensor view_of(const at::Tensor& buf, int64_t offset, at::IntArrayRef sizes) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(
+      c10::Storage(buf.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), buf.dtype());
+  impl->set_storage_offset(offset);
+  impl->set_sizes_contiguous(sizes);
+  return at::Tensor(std::move(impl));
+}
+
+std::vector<at::Tensor> step_tables(const at::Tensor& ctx_lens, const at::Tensor& q_lens,
+                                    const c10::optional<at::Tensor>& rows, at::Tensor& seq_tables,
+                                    const at::Tensor& new_blocks, int64_t num_tokens,
+                                    int64_t block_size, int64_t group, int64_t rows_per_tile,
+                                    int64_t num_decode, at::Tensor& err) {
   using namespace st;
-  const int64_t B = ctx_lens.numel(), W = block_tables.size(1);
-  for (const at::Tensor* t : {&ctx_lens, &q_lens, &new_blocks, (const at::Tensor*)&block_tables,
-                              (const at::Tensor*)&seq_lens, (const at::Tensor*)&cu_q,
-                              (const at::Tensor*)&positions, (const at::Tensor*)&slots,
-                              (const at::Tensor*)&last_rows, (const at::Tensor*)&tile_seq,
-                              (const at::Tensor*)&tile_row0, (const at::Tensor*)&num_new})
+  const int64_t B = ctx_lens.numel(), T = num_tokens;
+  for (const at::Tensor* t : {&ctx_lens, &q_lens, &new_blocks})
     TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kInt && t->is_contiguous(),
-                "step_tables: contiguous int32 CUDA tensors");
+                "step_tables: lengths and new_blocks are contiguous int32 CUDA tensors");
   TORCH_CHECK(seq_tables.is_cuda() && seq_tables.scalar_type() == at::kInt &&
-                  seq_tables.dim() == 2 && (seq_tables.size(1) <= 1 || seq_tables.stride(1) == 1) &&
-                  seq_tables.size(1) == W,
+                  seq_tables.dim() == 2 && (seq_tables.size(1) <= 1 || seq_tables.stride(1) == 1),
               "step_tables: seq_tables [S, W] int32, contiguous rows");
-  TORCH_CHECK(B >= 1 && B <= MAX_B, "step_tables: 1 to ", MAX_B, " requests");
-  TORCH_CHECK(q_lens.numel() == B && block_tables.size(0) == B && seq_lens.numel() == B &&
-                  cu_q.numel() == B + 1 && last_rows.numel() == B &&
-                  slots.numel() == positions.numel() && tile_row0.numel() == tile_seq.numel(),
-              "step_tables: sizes");
+  const int64_t W = seq_tables.size(1);
   const bool has_rows = rows.has_value() && rows->defined();
   if (has_rows)
     TORCH_CHECK(rows->is_cuda() && rows->scalar_type() == at::kInt && rows->is_contiguous() &&
                     rows->numel() == B,
                 "step_tables: rows [B] int32");
+  TORCH_CHECK(B >= 1 && B <= MAX_B && q_lens.numel() == B, "step_tables: 1 to ", MAX_B,
+              " requests");
   TORCH_CHECK(block_size >= 1 && block_size <= 1024 && (block_size & (block_size - 1)) == 0,
               "step_tables: power-of-two block size");
-  TORCH_CHECK(group >= 1 && rows_per_tile >= 1, "step_tables: group, rows_per_tile");
-  TORCH_CHECK(W * block_size < (int64_t(1) << 31), "step_tables: table width");
+  TORCH_CHECK(group >= 1 && rows_per_tile >= 1 && T >= 0, "step_tables: group, rows_per_tile");
+  TORCH_CHECK(W >= 1 && W * block_size < (int64_t(1) << 31) && T * group < (int64_t(1) << 31) &&
+                  B * W < (int64_t(1) << 31),
+              "step_tables: table width or token count");
+  const int64_t tiles = T * group / rows_per_tile + B;
+  // one allocation, every output on a 16-byte boundary
+  int64_t used = 0;
+  auto place = [&](int64_t n) {
+    const int64_t at = used;
+    used += (n + 3) / 4 * 4;
+    return at;
+  };
+  const int64_t o_tab = place(B * W), o_len = place(B), o_cu = place(B + 1), o_pos = place(T),
+                o_slot = place(T), o_last = place(B), o_ts = place(tiles), o_tr = place(tiles),
+                o_new = place(1);
+  at::Tensor buf = at::empty({used}, ctx_lens.options());
+  int* p = buf.data_ptr<int>();
   Args a;
   a.ctx = ctx_lens.data_ptr<int>();
   a.q = q_lens.data_ptr<int>();
@@ -237,28 +256,28 @@ void step_tables(const at::Tensor& ctx_lens, const at::Tensor& q_lens,
   a.seq_tables = seq_tables.data_ptr<int>();
   a.tab_stride = seq_tables.stride(0);
   a.new_blocks = new_blocks.data_ptr<int>();
-  a.block_tables = block_tables.data_ptr<int>();
-  a.seq_lens = seq_lens.data_ptr<int>();
-  a.cu_q = cu_q.data_ptr<int>();
-  a.positions = positions.data_ptr<int>();
-  a.slots = slots.data_ptr<int>();
-  a.last_rows = last_rows.data_ptr<int>();
-  a.tile_seq = tile_seq.data_ptr<int>();
-  a.tile_row0 = tile_row0.data_ptr<int>();
-  a.num_new = num_new.data_ptr<int>();
+  a.block_tables = p + o_tab;
+  a.seq_lens = p + o_len;
+  a.cu_q = p + o_cu;
+  a.positions = p + o_pos;
+  a.slots = p + o_slot;
+  a.last_rows = p + o_last;
+  a.tile_seq = p + o_ts;
+  a.tile_row0 = p + o_tr;
+  a.num_new = p + o_new;
   a.err = err.data_ptr<int>();
   a.B = B;
   a.S = seq_tables.size(0);
   a.W = W;
   a.F = new_blocks.numel();
-  a.T = positions.numel();
+  a.T = T;
   a.log2_bs = 0;
   while ((1 << a.log2_bs) < block_size) ++a.log2_bs;
   a.group = group;
   a.rows_per_tile = rows_per_tile;
-  a.num_tiles = tile_seq.numel();
+  a.num_tiles = tiles;
   a.num_decode = num_decode;
-  const int64_t items = std::max<int64_t>({B * 32, a.T, a.num_tiles, B * W / 8});
+  const int64_t items = std::max<int64_t>({B * ((W + SEG - 1) / SEG) * 32, T, tiles});
   const int grid = static_cast<int>(std::min<int64_t>(148, (items + THREADS - 1) / THREADS));
   const size_t smem = (4 * B + 3) * sizeof(int);
   if (smem > 48 * 1024)
@@ -267,6 +286,9 @@ void step_tables(const at::Tensor& ctx_lens, const at::Tensor& q_lens,
                                         static_cast<int>((4 * MAX_B + 3) * sizeof(int))));
   C10_CUDA_CHECK(launch_k(step_tables_kernel, dim3(grid), dim3(THREADS), smem,
                           at::cuda::getCurrentCUDAStream(), nullptr, 0, a));
+  return {view_of(buf, o_tab, {B, W}), view_of(buf, o_len, {B}), view_of(buf, o_cu, {B + 1}),
+          view_of(buf, o_pos, {T}), view_of(buf, o_slot, {T}), view_of(buf, o_last, {B}),
+          view_of(buf, o_ts, {tiles}), view_of(buf, o_tr, {tiles}), view_of(buf, o_new, {1})};
 }
 
 }  // namespace lb

@@ -59,30 +59,19 @@ def step_tables(ctx_lens: torch.Tensor, q_lens: torch.Tensor, rows: Optional[tor
         raise ValueError("step_tables: num_tokens, group, rows_per_tile")
     if block_size < 1 or block_size > 1024 or block_size & (block_size - 1):
         raise ValueError(f"step_tables: block size {block_size} is not a power of two up to 1024")
-    tiles = num_tokens * group // rows_per_tile + b
-    dev = ctx_lens.device
-    sizes = (b * w, b, b + 1, num_tokens, num_tokens, b, tiles, tiles, 1)
-    # one allocation; every output starts on a 16-byte boundary
-    starts, n = [], 0
-    for s in sizes:
-        starts.append(n)
-        n += (s + 3) // 4 * 4
-    buf = torch.empty(n, dtype=torch.int32, device=dev)
-    v = [buf[o:o + s] for o, s in zip(starts, sizes)]
-    out = StepTables(v[0].view(b, w), *v[1:])
     if ctx_lens.is_cuda:
-        _need_c().step_tables(ctx_lens, q_lens, rows, seq_tables, new_blocks, *out, block_size,
-                              group, rows_per_tile, num_decode, scratch(dev).err)
+        out = StepTables(*_need_c().step_tables(
+            ctx_lens, q_lens, rows, seq_tables, new_blocks, num_tokens, block_size, group,
+            rows_per_tile, num_decode, scratch(ctx_lens.device).err))
         _launches[0] += 1
         return out
+    tiles = num_tokens * group // rows_per_tile + b
+    out = StepTables(*(torch.zeros(n, dtype=torch.int32) for n in (
+        (b, w), b, b + 1, num_tokens, num_tokens, b, tiles, tiles, 1)))
     # CPU restatement
-    out.positions.zero_()
     out.slots.fill_(-1)
-    out.block_tables.zero_()
     out.tile_seq.fill_(-1)
-    out.tile_row0.zero_()
-    row = tok = used = tile = 0
-    out.cu_q[0] = 0
+    tok = used = tile = 0
     for i, (c, n) in enumerate(zip(ctx_lens.tolist(), q_lens.tolist())):
         row = i if rows is None else int(rows[i])
         if c < 0 or n < 0 or not 0 <= row < seq_tables.shape[0] or c + n > w * block_size:
