@@ -3,8 +3,8 @@
 //   s_j = scale * ks_{b(j)} * (q . k8_j),  p_j = exp(s_j - max s),
 //   o   = sum_j p_j vs_{b(j)} v8_j / sum_j p_j
 //
-// Argument checks and the choice of kernel: attn_fp8_decode.cu for one query token per sequence,
-// attn_fp8_prefill.cu (tcgen05) for the rest.
+// Argument checks and the choice of kernel: attn_fp8_rows.cu for one query token per sequence and
+// for work lists of few rows an item, attn_fp8_prefill.cu (tcgen05) for the rest.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -74,7 +74,9 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   if (decode) {
     TORCH_CHECK(q.size(0) >= B, op, ": one query token per sequence");
     if (B == 0) return;
-    fp8_decode(a, tk, tv, q, st);
+    TORCH_CHECK(fp8_rows_fits(a, false), op,
+                ": at most 4096 sequences, and 2^31 / 32 keys x KV heads in their tables");
+    fp8_rows(a, false, tk, tv, q, st);
     return;
   }
   TORCH_CHECK(cu_q.has_value() && tile_seq.has_value() && tile_row0.has_value(), op,
@@ -88,7 +90,13 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   a.tile_seq = tile_seq->data_ptr<int>();
   a.tile_row0 = tile_row0->data_ptr<int>();
   a.num_tiles = tile_seq->numel();
-  fp8_prefill(a, tk, tv, st);
+  // At most FEW_ROWS query rows per item on average (verification of a few tokens, tails of prompts):
+  // 256-row tiles would be mostly padding.
+  constexpr int64_t FEW_ROWS = 32;
+  if (q.size(0) * group <= FEW_ROWS * a.num_tiles && fp8_rows_fits(a, true))
+    fp8_rows(a, true, tk, tv, q, st);
+  else
+    fp8_prefill(a, tk, tv, st);
 }
 
 }  // namespace lb

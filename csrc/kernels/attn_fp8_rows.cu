@@ -1,24 +1,26 @@
-// Decode attention over the 8-bit paged KV cache (sm_100a): one query token per sequence.
+// Attention over the 8-bit paged KV cache for few query rows per sequence (sm_100a): decode (one
+// token) and short chunks such as speculative verification.
 //
 //   s_j = scale * ks_{b(j)} (q . k8_j),   m = max_j s_j,   p_j = 2^(s_j - m),  l = sum_j p_j
 //   o   = sum_j p_j vs_{b(j)} v8_j / l
 //
-// HBM-bound: every cache byte is used once per group of query heads, so the work is to keep
-// enough bytes in flight on every SM and to spend few instructions per byte.
+// HBM-bound: every cache byte is used once per few query rows, so the work is to keep enough bytes
+// in flight on every SM and to spend few instructions per byte.
 //
-// Work split.  The keys of all (sequence, KV head) pairs form one line of 32-key tiles; each
-// warp takes an equal, contiguous share of it (the sum over the lengths is repeated by every
-// CTA, so no host length and no plan is needed).  Ragged batches, a single long sequence and
-// many short ones all load the SMs evenly.  A pair that lies in one share is written at once; a
-// pair cut by share boundaries leaves (m, l, O) partials that a second kernel joins in order, so
-// results do not depend on timing.
+// Work split.  An entry is a sequence (decode) or an item of the work list; its query rows (token,
+// head in group) are cut into chunks of 8 or 16 columns, and (KV head, chunk) over the entry's keys
+// is a run of 32-key tiles.  All runs form one line; each warp takes an equal, contiguous share of
+// it (the sum over the lengths is repeated by every CTA, so no host length and no plan is needed).
+// Ragged batches, a single long sequence and many short ones all load the SMs evenly.  A run that
+// lies in one share is written at once; a run cut by share boundaries leaves (m, l, O) partials that
+// a second kernel joins in order, so results do not depend on timing.
 //
 // Each warp is its own pipeline: its lanes 0 and 1 issue the TMA loads of a tile's two 16-key
 // slices (K and V, 128-byte-swizzled rows) STAGES tiles ahead and its 32 lanes consume them;
 // no CTA barrier in the loop.
 //
 // Arithmetic.  The MMAs are transposed, S^T = K Q^T and O^T = V^T P^T, so that up to 8 query
-// heads are the n = 8 columns: half the MMAs and registers of heads padded to 16 rows.  K codes
+// rows are the n = 8 columns: half the MMAs and registers of rows padded to 16.  K codes
 // come out of ldmatrix four dims per register and V codes, with the transposing 8-bit ldmatrix,
 // four keys per register; the order of a contraction's index is free, so both feed the MMA after
 // one cvt per pair, with q and the keys permuted to match.  K's second 8-key group starts at key
@@ -42,14 +44,16 @@ constexpr int THREADS = 32 * WARPS;
 constexpr int STAGES = 3;
 constexpr int STAGE = 2 * 2 * SLICE;          // K slices, then V slices
 constexpr int WARP_SMEM = STAGES * STAGE;
-constexpr int MAX_SEQS = 4096;
+constexpr int MAX_ENTRIES = 4096;
+constexpr int ENTRY_ROWS = 256;               // packed query rows of a work list's item
+constexpr int MIN_TILES = 4;                  // per share: less is not worth a partial result
 constexpr float P_TOP = 32768.f;              // weights are p * 2^15
 
 struct Work {
-  float* part_o;      // [2 workers][heads of a chunk][D]
-  float2* part_ml;    // [2 workers][heads of a chunk]
+  float* part_o;      // [2 workers][columns of a chunk][D]
+  float2* part_ml;    // [2 workers][columns of a chunk]
   int workers;        // warps of the grid
-  int chunks;         // query-head chunks per KV head
+  int entries;
 };
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -90,24 +94,78 @@ __device__ __forceinline__ float sum_over_keys(float v) {
 // Key (within a slice) of row r of the S^T tile.
 __device__ __forceinline__ int key_of_row(int r) { return r < 8 ? r : 8 + ((r + 4) & 7); }
 
-// First tile of each sequence (s_cum, in units of one tile of one head chunk) and its length.
-// Every thread of the CTA takes part; the number of heads times chunks is `hc`.
-__device__ void scan_lengths(const Args& a, int hc, int* s_cum, int* s_len, int* s_tot) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int base = 0;
-  for (int b0 = 0; b0 < a.num_seqs; b0 += THREADS) {
-    const int b = b0 + tid;
-    int len = 0;
-    if (b < a.num_seqs) {
-      len = max(0, a.seq_lens[b]);
-      const int64_t cap = static_cast<int64_t>(a.bt_width) << a.log2_bs;
-      if (len > cap) {
-        record_error(a.err, kErrBounds);
-        len = static_cast<int>(cap);
-      }
-      s_len[b] = len;
+// What an entry is, in shared memory: first unit on the line, keys that its rows see; for a work
+// list also its runs, sequence, first query token and row, rows, and the keys before its first
+// token (token j of the sequence's new ones sees keys [0, lo + j]).
+template <bool LIST>
+struct Entries {
+  static constexpr int FIELDS = LIST ? 8 : 2;
+  int n;
+  int *cum, *lim, *runs, *seq, *q0, *row0, *rows, *lo;
+  __device__ Entries(int* base, int n_) : n(n_) {
+    cum = base;                                  // n + 1
+    lim = cum + n + 1;
+    if (LIST) {
+      runs = lim + n;
+      seq = runs + n;
+      q0 = seq + n;
+      row0 = q0 + n;
+      rows = row0 + n;
+      lo = rows + n;
     }
-    int v = (len + KT - 1) / KT * hc;
+  }
+  static size_t bytes(int n) { return (static_cast<size_t>(FIELDS) * n + 1) * sizeof(int); }
+};
+
+// Fills the entries; every thread of the CTA takes part.  HT: columns per chunk.
+template <bool LIST, int HT>
+__device__ void scan_entries(const Args& a, const Entries<LIST>& en, int* s_tot) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t cap = static_cast<int64_t>(a.bt_width) << a.log2_bs;
+  int base = 0;
+  for (int e0 = 0; e0 < en.n; e0 += THREADS) {
+    const int e = e0 + tid;
+    int lim = 0, runs = a.hkv * ((a.group + HT - 1) / HT);
+    if (e < en.n) {
+      int seq = e;
+      if (LIST) {
+        seq = a.tile_seq[e];
+        const int row0 = a.tile_row0[e];
+        if (seq >= a.num_seqs || row0 < 0) {
+          record_error(a.err, kErrBounds);
+          seq = -1;
+        }
+        int q0 = 0, rows = 0, lo = 0;
+        if (seq >= 0) {
+          q0 = a.cu_q[seq];
+          const int n = a.cu_q[seq + 1] - q0;
+          rows = max(0, min(n * a.group - row0, ENTRY_ROWS));
+          lim = max(0, a.seq_lens[seq]);
+          if (lim > cap) {
+            record_error(a.err, kErrBounds);
+            lim = static_cast<int>(cap);
+          }
+          lo = a.causal ? lim - n : 0x3fffffff;
+          if (a.causal) lim = max(0, min(lim, lo + (row0 + rows - 1) / a.group + 1));
+          if (rows == 0) lim = 0;
+        }
+        runs = a.hkv * ((rows + HT - 1) / HT);
+        en.runs[e] = runs;
+        en.seq[e] = seq;
+        en.q0[e] = q0;
+        en.row0[e] = row0;
+        en.rows[e] = rows;
+        en.lo[e] = lo;
+      } else {
+        lim = max(0, a.seq_lens[seq]);
+        if (lim > cap) {
+          record_error(a.err, kErrBounds);
+          lim = static_cast<int>(cap);
+        }
+      }
+      en.lim[e] = lim;
+    }
+    int v = (lim + KT - 1) / KT * runs;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, v, o);
@@ -120,60 +178,77 @@ __device__ void scan_lengths(const Args& a, int hc, int* s_cum, int* s_len, int*
       if (w < warp) v += s_tot[w];
       all += s_tot[w];
     }
-    if (b < a.num_seqs) s_cum[b + 1] = base + v;
-    if (tid == 0 && b0 == 0) s_cum[0] = 0;
+    if (e < en.n) en.cum[e + 1] = base + v;
+    if (e == 0) en.cum[0] = 0;
     base += all;
     __syncthreads();
   }
 }
 
-// Shares: worker w of n takes units [w U / n, (w + 1) U / n).  Fewer than two tiles a worker is
-// not worth a partial result.
+// Shares: worker w of n takes units [w U / n, (w + 1) U / n).
 __device__ __forceinline__ int active_workers(int units, int workers) {
-  return max(1, min(workers, units / 2));
+  return max(1, min(workers, units / MIN_TILES));
 }
 __device__ __forceinline__ int share_begin(int w, int units, int n) {
   return static_cast<int>(static_cast<int64_t>(w) * units / n);
 }
-__device__ __forceinline__ int share_of(int unit, int units, int n) {
-  return static_cast<int>(((static_cast<int64_t>(unit) + 1) * n - 1) / units);
-}
 
 // A position on the line of tiles.
+template <bool LIST>
 struct Cursor {
-  int b, h, t, nt;   // sequence, head chunk, tile, tiles of the sequence
-  __device__ void seek(const int* cum, int n_seqs, int hc, int unit) {
-    int lo = 0, hi = n_seqs;
+  int e, r, t, nt;   // entry, run, tile, tiles of a run
+  __device__ void seek(const Entries<LIST>& en, int unit) {
+    int lo = 0, hi = en.n;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (cum[mid] <= unit) lo = mid;
+      if (en.cum[mid] <= unit) lo = mid;
       else hi = mid;
     }
-    b = lo;
-    nt = (cum[b + 1] - cum[b]) / hc;
-    const int r = unit - cum[b];
-    h = r / nt;
-    t = r - h * nt;
+    e = lo;
+    nt = (en.lim[e] + KT - 1) / KT;
+    const int x = unit - en.cum[e];
+    r = x / nt;
+    t = x - r * nt;
   }
   // to the next tile; only called when one exists
-  __device__ void next(const int* cum, int hc) {
+  __device__ void next(const Entries<LIST>& en, int runs) {
     if (++t < nt) return;
     t = 0;
-    if (++h < hc) return;
-    h = 0;
-    do {
-      ++b;
-      nt = cum[b + 1] - cum[b];
-    } while (nt == 0);
-    nt /= hc;
+    if (++r < (LIST ? en.runs[e] : runs)) return;
+    r = 0;
+    do ++e;
+    while (en.cum[e + 1] == en.cum[e]);
+    nt = (en.lim[e] + KT - 1) / KT;
   }
 };
 
-template <int NT>   // query-head tiles of 8 per chunk
+// The query rows of a run: column i is packed row `row + i` of the sequence's new tokens.
+struct Columns {
+  int kvh, seq, row, count, lo;
+  int64_t q0;                  // first query token of the sequence
+};
+template <bool LIST, int HT>
+__device__ __forceinline__ Columns columns_of(const Args& a, const Entries<LIST>& en,
+                                              const Cursor<LIST>& c) {
+  const int runs = LIST ? en.runs[c.e] : a.hkv * ((a.group + HT - 1) / HT);
+  const int chunks = runs / a.hkv;
+  Columns k;
+  k.kvh = c.r / chunks;
+  const int chunk = c.r - k.kvh * chunks;
+  const int rows = LIST ? en.rows[c.e] : a.group;
+  k.seq = LIST ? en.seq[c.e] : c.e;
+  k.row = (LIST ? en.row0[c.e] : 0) + chunk * HT;
+  k.count = min(HT, rows - chunk * HT);
+  k.lo = LIST ? en.lo[c.e] : 0x3fffffff;
+  k.q0 = LIST ? en.q0[c.e] : c.e;
+  return k;
+}
+
+template <bool LIST, int NT>   // NT: column tiles of 8 per chunk
 __global__ void __launch_bounds__(THREADS, 2)
-    decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                  const Args a, const Work wk) {
-  constexpr int HT = 8 * NT;                  // heads per chunk
+    rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                const Args a, const Work wk) {
+  constexpr int HT = 8 * NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -184,8 +259,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   float* s_scale = reinterpret_cast<float*>(smem + WARPS * WARP_SMEM + WARPS * STAGES * 8) +
                    warp * STAGES * 4;
   int* s_tot = reinterpret_cast<int*>(smem + WARPS * WARP_SMEM + WARPS * STAGES * 24);
-  int* s_cum = s_tot + WARPS;
-  int* s_len = s_cum + a.num_seqs + 1;
+  const Entries<LIST> en(s_tot + WARPS, wk.entries);
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 3);   // lane 0's expect + two scale loads
     fence_barrier_init();
@@ -195,10 +269,21 @@ __global__ void __launch_bounds__(THREADS, 2)
   __syncwarp();
   pdl_trigger();
   pdl_wait();
-  const int hc = a.hkv * wk.chunks;
-  scan_lengths(a, hc, s_cum, s_len, s_tot);
-  const int units = s_cum[a.num_seqs];
+  scan_entries<LIST, HT>(a, en, s_tot);
+  // rows that see no key give 0
+  for (int e = blockIdx.x; e < en.n; e += gridDim.x) {
+    if (en.lim[e] > 0) continue;                                    // CTA-uniform
+    const int row0 = LIST ? en.row0[e] : 0, rows = LIST ? en.rows[e] : a.group;
+    for (int i = threadIdx.x; i < rows * a.hkv * (D / 8); i += THREADS) {
+      const int c = i % (D / 8), x = i / (D / 8), r = row0 + x % rows, kvh = x / rows;
+      *reinterpret_cast<uint4*>(a.out + (LIST ? en.q0[e] + r / a.group : e) * a.out_ld +
+                                static_cast<int64_t>(kvh * a.group + r % a.group) * D + c * 8) =
+          make_uint4(0, 0, 0, 0);
+    }
+  }
+  const int units = en.cum[en.n];
   if (units == 0) return;
+  const int runs = a.hkv * ((a.group + HT - 1) / HT);   // of a decode entry
   const int n_act = active_workers(units, wk.workers);
   const int w = warp * gridDim.x + blockIdx.x;   // neighbours on the line sit on different SMs
   if (w >= n_act) return;
@@ -209,17 +294,23 @@ __global__ void __launch_bounds__(THREADS, 2)
   const uint64_t pol = policy_evict_first();
   // ---- producer state: lanes 0 and 1 own the tile's slices; the block id of the next tile to
   // issue is fetched one tile early ----
-  Cursor pc;
-  pc.seek(s_cum, a.num_seqs, hc, u_begin);
+  Cursor<LIST> pc;
+  pc.seek(en, u_begin);
+  auto place = [&](int& seq, int& kvh) {
+    seq = LIST ? en.seq[pc.e] : pc.e;
+    kvh = pc.r / ((LIST ? en.runs[pc.e] : runs) / a.hkv);
+  };
+  int p_seq, p_kvh;
+  place(p_seq, p_kvh);
   int pu = u_begin, p_id = 0;
   auto fetch_id = [&]() {
     const int key = pc.t * KT + lane * SL;
-    if (lane < 2 && pu < u_end && key < s_len[pc.b])
-      p_id = a.tables[pc.b * a.bt_stride + (key >> a.log2_bs)];
+    if (lane < 2 && pu < u_end && key < en.lim[pc.e])
+      p_id = a.tables[p_seq * a.bt_stride + (key >> a.log2_bs)];
   };
   auto issue = [&](int stage) {
     if (pu >= u_end) return;                                       // warp-uniform
-    const int key0 = pc.t * KT, len = s_len[pc.b];
+    const int key0 = pc.t * KT, len = en.lim[pc.e];
     if (lane == 0)
       mbar_arrive_expect_tx(&full[stage], (len - key0 > SL ? 2 : 1) * 2 * SLICE);
     __syncwarp();
@@ -227,7 +318,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       const int key = key0 + lane * SL;
       if (key < len) {
         const int blk = checked_block(a, p_id);
-        const int bh = blk * a.hkv + pc.h / wk.chunks;
+        const int bh = blk * a.hkv + p_kvh;
         const int row = (bh << a.log2_bs) + (key & ((1 << a.log2_bs) - 1));
         uint8_t* dst = ring + stage * STAGE + lane * SLICE;
         tma_load_2d(dst, &tmK, &full[stage], 0, row, pol);
@@ -243,7 +334,8 @@ __global__ void __launch_bounds__(THREADS, 2)
                    : "memory");
     }
     if (++pu < u_end) {
-      pc.next(s_cum, hc);
+      pc.next(en, runs);
+      if (pc.t == 0) place(p_seq, p_kvh);
       fetch_id();
     }
   };
@@ -251,8 +343,8 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll 1
   for (int s = 0; s < STAGES; ++s) issue(s);
 
-  Cursor cc;
-  cc.seek(s_cum, a.num_seqs, hc, u_begin);
+  Cursor<LIST> cc;
+  cc.seek(en, u_begin);
   // row addresses of the two ldmatrix shapes
   const int krow = key_of_row(((lane >> 3) & 1) * 8 + (lane & 7));
   const int kchunk = lane >> 4;
@@ -265,17 +357,31 @@ __global__ void __launch_bounds__(THREADS, 2)
   int u = u_begin, used = u_begin;               // used: tiles consumed, segment by segment u
   bool ok = true;
   while (u < u_end) {
-    // ---- one (sequence, head chunk): tiles [t0, t1) ----
-    const int t0 = cc.t, t1 = min(cc.nt, t0 + u_end - u), len = s_len[cc.b];
-    const int kvh = cc.h / wk.chunks, head0 = kvh * a.group + (cc.h % wk.chunks) * HT;
-    const int heads = min(HT, (kvh + 1) * a.group - head0);
+    // ---- tiles [t0, t1) of one run ----
+    const int t0 = cc.t, t1 = min(cc.nt, t0 + u_end - u), len = en.lim[cc.e];
+    const Columns co = columns_of<LIST, HT>(a, en, cc);
     uint32_t qf[NT][8][2];
     float hs[NT][2];
+    // where column i's row lies in q and out, and the keys that it sees
+    auto token_of = [&](int i) { return LIST ? (co.row + i) / a.group : 0; };
+    auto head_of = [&](int i) {
+      return co.kvh * a.group + (LIST ? (co.row + i) % a.group : co.row + i);
+    };
+    int see[NT][2], see_min = len;
+    if (LIST) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) see[n][j] = co.lo + token_of(n * 8 + 2 * t4 + j) + 1;
+      see_min = min(len, co.lo + token_of(0) + 1);
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       uint2 raw[8];
-      const bool have = n * 8 + g < heads;
-      const bf16* qp = a.q + cc.b * a.q_ld + static_cast<int64_t>(head0 + n * 8 + g) * D + t4 * 4;
+      const int col = n * 8 + g;
+      const bool have = col < co.count;
+      const bf16* qp = a.q + (co.q0 + token_of(col)) * a.q_ld +
+                       static_cast<int64_t>(head_of(col)) * D + t4 * 4;
       float amax = 0.f;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
@@ -352,15 +458,19 @@ __global__ void __launch_bounds__(THREADS, 2)
           s[i][n][3] *= ks * hs[n][1];
         }
       }
-      if (left < KT) {
-        // keys past the end: whatever their memory holds, their score is -inf
+      if (see_min - t * KT < KT) {
+        // keys that a row does not see, or past the end: whatever their memory holds, their score
+        // is -inf
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (i * SL + g >= left) s[i][n][0] = s[i][n][1] = -INFINITY;
-            if (i * SL + key_of_row(8 + g) >= left) s[i][n][2] = s[i][n][3] = -INFINITY;
-          }
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int key = i * SL + (x < 2 ? g : key_of_row(8 + g));
+              const int lim = LIST ? min(len, see[n][x & 1]) - t * KT : left;
+              if (key >= lim) s[i][n][x] = -INFINITY;
+            }
       }
       // ---- running maximum and sum ----
       float corr[NT][2];
@@ -457,16 +567,16 @@ __global__ void __launch_bounds__(THREADS, 2)
       const int h0 = n * 8 + 2 * t4;
       if (whole) {
         const float i0 = l0 != 0.f ? vmul / l0 : 0.f, i1 = l1 != 0.f ? vmul / l1 : 0.f;
-        bf16* dst = a.out + cc.b * a.out_ld + static_cast<int64_t>(head0 + h0) * D + g;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          if (h0 < heads) {
-            dst[d * 16] = __float2bfloat16(o[n][d][0] * i0);
-            dst[d * 16 + 8] = __float2bfloat16(o[n][d][2] * i0);
-          }
-          if (h0 + 1 < heads) {
-            dst[D + d * 16] = __float2bfloat16(o[n][d][1] * i1);
-            dst[D + d * 16 + 8] = __float2bfloat16(o[n][d][3] * i1);
+        for (int j = 0; j < 2; ++j) {
+          if (h0 + j >= co.count) continue;
+          bf16* dst = a.out + (co.q0 + token_of(h0 + j)) * a.out_ld +
+                      static_cast<int64_t>(head_of(h0 + j)) * D + g;
+          const float inv = j ? i1 : i0;
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            dst[d * 16] = __float2bfloat16(o[n][d][j] * inv);
+            dst[d * 16 + 8] = __float2bfloat16(o[n][d][j + 2] * inv);
           }
         }
       } else {
@@ -487,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     u += t1 - t0;
     if (u < u_end) {
       cc.t = cc.nt - 1;
-      cc.next(s_cum, hc);
+      cc.next(en, runs);
     }
   }
   if (!ok) {
@@ -504,101 +614,135 @@ __global__ void __launch_bounds__(THREADS, 2)
   }
 }
 
-// Joins the parts of the pairs that share boundaries cut, in the order of the keys; sequences
-// without a key give 0.  One warp per (sequence, query head), 4 dims per lane.
-template <int NT>
+// Joins the parts of the runs that share boundaries cut, in the order of the keys.  One warp per
+// (share, column): the share that a cut run starts in owns it.  The parts' maxima and sums are read
+// by the lanes together, their O rows (4 dims per lane) eight at a time.
+template <bool LIST, int NT>
 __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const Work wk) {
   constexpr int HT = 8 * NT;
   extern __shared__ int smem_i[];
   int* s_tot = smem_i;
-  int* s_cum = s_tot + WARPS;
-  int* s_len = s_cum + a.num_seqs + 1;
+  const Entries<LIST> en(s_tot + WARPS, wk.entries);
   pdl_trigger();
   pdl_wait();
-  const int hc = a.hkv * wk.chunks;
-  scan_lengths(a, hc, s_cum, s_len, s_tot);
-  const int units = s_cum[a.num_seqs];
+  scan_entries<LIST, HT>(a, en, s_tot);
+  const int units = en.cum[en.n];
   const int n_act = active_workers(units, wk.workers);
   const int lane = threadIdx.x & 31;
-  const int64_t rows = static_cast<int64_t>(a.num_seqs) * a.hq;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * WARPS + (threadIdx.x >> 5); i < rows;
-       i += static_cast<int64_t>(gridDim.x) * WARPS) {
-    const int b = static_cast<int>(i / a.hq), head = static_cast<int>(i % a.hq);
-    const int nt = (s_cum[b + 1] - s_cum[b]) / hc;
-    float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, m = -INFINITY;
-    if (nt > 0) {
-      const int kvh = head / a.group, in = head % a.group;
-      const int ua = s_cum[b] + (kvh * wk.chunks + in / HT) * nt, ub = ua + nt;
-      const int wa = share_of(ua, units, n_act), wb = share_of(ub - 1, units, n_act);
-      if (wa == wb) continue;                       // written whole by its warp
-      const bool starts = share_begin(wa, units, n_act) <= ua;
-      for (int w = wa; w <= wb; ++w) {
-        const int64_t row = static_cast<int64_t>(2 * w + (w == wa && starts ? 1 : 0)) * HT + in % HT;
-        const float2 ml = wk.part_ml[row];
-        const float4 v = *reinterpret_cast<const float4*>(wk.part_o + row * D + lane * 4);
-        const float mn = fmaxf(m, ml.x);
-        const float safe = mn == -INFINITY ? 0.f : mn;
-        const float c0 = ex2(m - safe), c1 = ex2(ml.x - safe);
-        m = mn;
-        l = l * c0 + ml.y * c1;
-        o[0] = o[0] * c0 + v.x * c1;
-        o[1] = o[1] * c0 + v.y * c1;
-        o[2] = o[2] * c0 + v.z * c1;
-        o[3] = o[3] * c0 + v.w * c1;
+  for (int i = blockIdx.x * WARPS + (threadIdx.x >> 5); i < n_act * HT; i += gridDim.x * WARPS) {
+    const int w = i / HT, col = i % HT;
+    const int end = share_begin(w + 1, units, n_act);
+    if (end >= units) continue;                     // the line ends here: nothing is cut
+    Cursor<LIST> c;
+    c.seek(en, end);
+    const int u0 = end - c.t, u1 = u0 + c.nt;       // the run that holds the next share's first tile
+    if (c.t == 0 || u0 < share_begin(w, units, n_act)) continue;   // not cut, or not ours
+    const Columns co = columns_of<LIST, HT>(a, en, c);
+    if (col >= co.count) continue;
+    // parts: slot 2 w + 1, then 2 (w + 1), 2 (w + 2), ... while shares start inside the run
+    int parts = 1;
+    while (share_begin(w + parts, units, n_act) < u1 && w + parts < n_act) ++parts;
+    auto row_of = [&](int k) {
+      return static_cast<int64_t>(k == 0 ? 2 * w + 1 : 2 * (w + k)) * HT + col;
+    };
+    float m = -INFINITY;
+    for (int k = lane; k < parts; k += 32) m = fmaxf(m, wk.part_ml[row_of(k)].x);
+    m = warp_max(m);
+    const float safe = m == -INFINITY ? 0.f : m;
+    float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+      float f = 0.f;
+      if (k0 + lane < parts) {
+        const float2 ml = wk.part_ml[row_of(k0 + lane)];
+        f = ex2(ml.x - safe);
+        l += ml.y * f;
+      }
+      const int n = min(32, parts - k0);
+      for (int k = 0; k < n; k += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          v[x] = k + x < n ? *reinterpret_cast<const float4*>(wk.part_o + row_of(k0 + k + x) * D +
+                                                              lane * 4)
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float c1 = __shfl_sync(0xffffffffu, f, (k + x) & 31);
+          if (k + x < n) {
+            o[0] += v[x].x * c1;
+            o[1] += v[x].y * c1;
+            o[2] += v[x].z * c1;
+            o[3] += v[x].w * c1;
+          }
+        }
       }
     }
+    l = warp_sum(l);
     const float inv = l != 0.f ? 1.f / l : 0.f;
-    *reinterpret_cast<uint2*>(a.out + b * a.out_ld + static_cast<int64_t>(head) * D + lane * 4) =
+    const int tok = LIST ? (co.row + col) / a.group : 0;
+    const int head = co.kvh * a.group + (LIST ? (co.row + col) % a.group : co.row + col);
+    *reinterpret_cast<uint2*>(a.out + (co.q0 + tok) * a.out_ld + static_cast<int64_t>(head) * D +
+                              lane * 4) =
         make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
   }
 }
 
-template <int NT>
+// Upper bound of the line's length.
+static int64_t line_bound(const Args& a, bool list, int ht) {
+  const int64_t rows = list ? ENTRY_ROWS : a.group;
+  return (list ? a.num_tiles : a.num_seqs) * static_cast<int64_t>(a.hkv) * ((rows + ht - 1) / ht) *
+         (((static_cast<int64_t>(a.bt_width) << a.log2_bs) + KT - 1) / KT);
+}
+
+template <bool LIST, int NT>
 void launch(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const at::Tensor& like,
             cudaStream_t st) {
   constexpr int HT = 8 * NT;
-  const size_t lens = (WARPS + 2 * static_cast<size_t>(a.num_seqs) + 1) * sizeof(int);
+  Work wk;
+  wk.entries = LIST ? a.num_tiles : a.num_seqs;
+  const size_t lens = WARPS * sizeof(int) + Entries<LIST>::bytes(wk.entries);
   const size_t smem = 1024 + WARPS * WARP_SMEM + WARPS * STAGES * 24 + lens;
   static bool attr = false;
   if (!attr) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(decode_kernel<NT>,
+    C10_CUDA_CHECK(cudaFuncSetAttribute(rows_kernel<LIST, NT>,
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    C10_CUDA_CHECK(cudaFuncSetAttribute(join_kernel<LIST, NT>,
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     attr = true;
   }
-  Work wk;
-  wk.chunks = (a.group + HT - 1) / HT;
-  // two CTAs an SM while both fit (beyond about 2000 sequences the length tables leave room for
-  // one); no more warps than tiles there can be
-  const int per_sm = 2 * smem <= 226 * 1024 ? 2 : 1;
-  const int64_t tiles = static_cast<int64_t>(a.num_seqs) * a.hkv * wk.chunks *
-                        (((static_cast<int64_t>(a.bt_width) << a.log2_bs) + KT - 1) / KT);
+  // two CTAs an SM while both fit (the entries' tables of a very large batch leave room for one); no
+  // more warps than the tiles there can be make shares
+  const int per_sm = 2 * (smem + 1024) <= 228 * 1024 ? 2 : 1;
+  const int64_t tiles = line_bound(a, LIST, HT);
   const int grid = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>(148 * per_sm, (tiles + 1) / 2)));
+      std::max<int64_t>(1, std::min<int64_t>(148 * per_sm, (tiles + MIN_TILES - 1) / MIN_TILES)));
   wk.workers = grid * WARPS;
   at::Tensor ws = at::empty({static_cast<int64_t>(wk.workers) * 2 * HT * (D + 2)},
                             like.options().dtype(at::kFloat));
   wk.part_o = ws.data_ptr<float>();
   wk.part_ml = reinterpret_cast<float2*>(wk.part_o + static_cast<int64_t>(wk.workers) * 2 * HT * D);
-  C10_CUDA_CHECK(launch_k(decode_kernel<NT>, dim3(grid), dim3(THREADS), smem, st, nullptr, 0, tk,
-                          tv, a, wk));
-  const int64_t rows = static_cast<int64_t>(a.num_seqs) * a.hq;
-  C10_CUDA_CHECK(launch_k(join_kernel<NT>,
-                          dim3(static_cast<int>(std::min<int64_t>((rows + WARPS - 1) / WARPS, 1184))),
-                          dim3(THREADS), lens, st, nullptr, 0, a, wk));
+  auto rk = rows_kernel<LIST, NT>;
+  auto jk = join_kernel<LIST, NT>;
+  C10_CUDA_CHECK(launch_k(rk, dim3(grid), dim3(THREADS), smem, st, nullptr, 0, tk, tv, a, wk));
+  const int jgrid = std::min(wk.workers * HT / WARPS, 148 * 8);
+  C10_CUDA_CHECK(launch_k(jk, dim3(std::max(1, jgrid)), dim3(THREADS), lens, st, nullptr, 0, a, wk));
 }
 
 }  // namespace fp8d
 
-void fp8_decode(const fp8a::Args& a, const CUtensorMap& tk, const CUtensorMap& tv,
-                const at::Tensor& like, cudaStream_t st) {
-  TORCH_CHECK(a.num_seqs <= fp8d::MAX_SEQS, "paged_attention_fp8: at most ", fp8d::MAX_SEQS,
-              " sequences");
-  TORCH_CHECK(static_cast<int64_t>(a.num_seqs) * a.hq *
-                      ((static_cast<int64_t>(a.bt_width) << a.log2_bs) / fp8d::KT + 1) <
-                  (int64_t(1) << 31),
-              "paged_attention_fp8: sequences x heads x table width too large");
-  if (a.group <= 8) fp8d::launch<1>(a, tk, tv, like, st);
-  else fp8d::launch<2>(a, tk, tv, like, st);
+bool fp8_rows_fits(const fp8a::Args& a, bool list) {
+  return (list ? a.num_tiles : a.num_seqs) <= fp8d::MAX_ENTRIES &&
+         fp8d::line_bound(a, list, 8) < (int64_t(1) << 31);
+}
+
+void fp8_rows(const fp8a::Args& a, bool list, const CUtensorMap& tk, const CUtensorMap& tv,
+              const at::Tensor& like, cudaStream_t st) {
+  using namespace fp8d;
+  // decode: a group of up to 8 heads fills one column tile; a list's rows are (token, head) pairs,
+  // usually more than 8
+  if (list) launch<true, 2>(a, tk, tv, like, st);
+  else if (a.group <= 8) launch<false, 1>(a, tk, tv, like, st);
+  else launch<false, 2>(a, tk, tv, like, st);
 }
 
 }  // namespace lb
