@@ -31,6 +31,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 
+#include <type_traits>
+
 #include "attn_fp8.cuh"
 
 namespace lb {
@@ -41,15 +43,25 @@ using namespace fp8a;
 constexpr int KT = 32;                        // keys per tile
 constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
-constexpr int STAGES = 3;
 constexpr int STAGE = 2 * 2 * SLICE;          // K slices, then V slices
-constexpr int WARP_SMEM = STAGES * STAGE;
+// One column tile: 2 stages and 12 warps an SM; two: 3 stages and 8 warps (their O takes twice the
+// registers).  Both keep 192 KB of an SM in flight.
+constexpr int stages_of(int nt) { return nt == 1 ? 2 : 3; }
+constexpr int ctas_of(int nt) { return nt == 1 ? 3 : 2; }
 constexpr int MAX_ENTRIES = 4096;
 constexpr int ENTRY_ROWS = 256;               // packed query rows of a work list's item
 constexpr int MIN_TILES = 4;                  // per share: less is not worth a partial result
 constexpr float P_TOP = 32768.f;              // weights are p * 2^15
 
+// A run that starts in a share and goes on in the next ones, for the kernel that joins its parts.
+struct Cut {
+  int parts;          // 0: the share has none
+  int count, row, kvh;
+  int64_t q0;
+};
+
 struct Work {
+  Cut* cut;           // [workers]
   float* part_o;      // [2 workers][columns of a chunk][D]
   float2* part_ml;    // [2 workers][columns of a chunk]
   int workers;        // warps of the grid
@@ -192,6 +204,9 @@ __device__ __forceinline__ int active_workers(int units, int workers) {
 __device__ __forceinline__ int share_begin(int w, int units, int n) {
   return static_cast<int>(static_cast<int64_t>(w) * units / n);
 }
+__device__ __forceinline__ int share_of(int unit, int units, int n) {
+  return static_cast<int>(((static_cast<int64_t>(unit) + 1) * n - 1) / units);
+}
 
 // A position on the line of tiles.
 template <bool LIST>
@@ -245,10 +260,10 @@ __device__ __forceinline__ Columns columns_of(const Args& a, const Entries<LIST>
 }
 
 template <bool LIST, int NT>   // NT: column tiles of 8 per chunk
-__global__ void __launch_bounds__(THREADS, 2)
+__global__ void __launch_bounds__(THREADS, ctas_of(NT))
     rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                 const Args a, const Work wk) {
-  constexpr int HT = 8 * NT;
+  constexpr int HT = 8 * NT, STAGES = stages_of(NT), WARP_SMEM = STAGES * STAGE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -268,7 +283,8 @@ __global__ void __launch_bounds__(THREADS, 2)
   }
   __syncwarp();
   pdl_trigger();
-  pdl_wait();
+  const int w = warp * gridDim.x + blockIdx.x;   // neighbours on the line sit on different SMs
+  if (lane == 0) wk.cut[w].parts = 0;
   scan_entries<LIST, HT>(a, en, s_tot);
   // rows that see no key give 0
   for (int e = blockIdx.x; e < en.n; e += gridDim.x) {
@@ -285,7 +301,6 @@ __global__ void __launch_bounds__(THREADS, 2)
   if (units == 0) return;
   const int runs = a.hkv * ((a.group + HT - 1) / HT);   // of a decode entry
   const int n_act = active_workers(units, wk.workers);
-  const int w = warp * gridDim.x + blockIdx.x;   // neighbours on the line sit on different SMs
   if (w >= n_act) return;
   const int u_begin = share_begin(w, units, n_act), u_end = share_begin(w + 1, units, n_act);
   if (u_begin >= u_end) return;
@@ -524,27 +539,33 @@ __global__ void __launch_bounds__(THREADS, 2)
             p[n][0] = transpose8(pack_f16x2(s[i][n][0] * c, s[i][n][1] * c));
             p[n][1] = transpose8(pack_f16x2(s[i][n][2] * c, s[i][n][3] * c));
           }
-          // codes of keys past the end become zeros (NaN times weight 0 would be NaN)
-          uint32_t keep = 0xffffffffu;
-          if (left - i * SL < SL) {
-            keep = 0;
+          const uint32_t base = v_addr + stage * STAGE + i * SLICE;
+          auto add_v = [&](auto masked, uint32_t keep) {
+#pragma unroll
+            for (int c2 = 0; c2 < 8; c2 += 2) {
+              uint32_t r[4], x[4];
+              ldsm_t8(r, base + (((c2 + kchunk) ^ (vrow & 7)) << 4));
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t lo = masked ? r[2 * e] & keep : r[2 * e];
+                const uint32_t hi = masked ? r[2 * e + 1] & keep : r[2 * e + 1];
+                e4m3x4_to_f16(lo, x[0], x[2]);
+                e4m3x4_to_f16(hi, x[1], x[3]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                  mma_f16(o[n][c2 + e], x[0], x[1], x[2], x[3], p[n][0], p[n][1]);
+              }
+            }
+          };
+          if (left - i * SL >= SL) {
+            add_v(std::false_type{}, 0u);
+          } else {
+            // codes of keys past the end become zeros (NaN times weight 0 would be NaN)
+            uint32_t keep = 0;
 #pragma unroll
             for (int y = 0; y < 4; ++y)
               if (key_of_row(2 * t4 + (y & 1) + (y & 2) * 4) < left - i * SL) keep |= 0xffu << (8 * y);
-          }
-          const uint32_t base = v_addr + stage * STAGE + i * SLICE;
-#pragma unroll
-          for (int c2 = 0; c2 < 8; c2 += 2) {
-            uint32_t r[4], x[4];
-            ldsm_t8(r, base + (((c2 + kchunk) ^ (vrow & 7)) << 4));
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              e4m3x4_to_f16(r[2 * e] & keep, x[0], x[2]);
-              e4m3x4_to_f16(r[2 * e + 1] & keep, x[1], x[3]);
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-                mma_f16(o[n][c2 + e], x[0], x[1], x[2], x[3], p[n][0], p[n][1]);
-            }
+            add_v(std::true_type{}, keep);
           }
         }
       }
@@ -560,6 +581,8 @@ __global__ void __launch_bounds__(THREADS, 2)
     // ---- the pair's result, or this share's part of it ----
     const bool whole = t0 == 0 && t1 == cc.nt;
     const int slot = 2 * w + (t0 == 0 ? 1 : 0);
+    if (t0 == 0 && !whole && lane == 0)
+      wk.cut[w] = Cut{share_of(u + cc.nt - 1, units, n_act) - w + 1, co.count, co.row, co.kvh, co.q0};
     const float vmul = vref * (1.f / P_TOP);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -615,76 +638,61 @@ __global__ void __launch_bounds__(THREADS, 2)
 }
 
 // Joins the parts of the runs that share boundaries cut, in the order of the keys.  One warp per
-// (share, column): the share that a cut run starts in owns it.  The parts' maxima and sums are read
-// by the lanes together, their O rows (4 dims per lane) eight at a time.
+// (share, column): the share that a cut run starts in describes it.  The parts' maxima and sums are
+// read by the lanes together, their O rows (4 dims per lane) eight at a time.
 template <bool LIST, int NT>
 __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const Work wk) {
   constexpr int HT = 8 * NT;
-  extern __shared__ int smem_i[];
-  int* s_tot = smem_i;
-  const Entries<LIST> en(s_tot + WARPS, wk.entries);
+  const int lane = threadIdx.x & 31;
+  const int i = blockIdx.x * WARPS + (threadIdx.x >> 5);
+  const int w = i / HT, col = i % HT;
   pdl_trigger();
   pdl_wait();
-  scan_entries<LIST, HT>(a, en, s_tot);
-  const int units = en.cum[en.n];
-  const int n_act = active_workers(units, wk.workers);
-  const int lane = threadIdx.x & 31;
-  for (int i = blockIdx.x * WARPS + (threadIdx.x >> 5); i < n_act * HT; i += gridDim.x * WARPS) {
-    const int w = i / HT, col = i % HT;
-    const int end = share_begin(w + 1, units, n_act);
-    if (end >= units) continue;                     // the line ends here: nothing is cut
-    Cursor<LIST> c;
-    c.seek(en, end);
-    const int u0 = end - c.t, u1 = u0 + c.nt;       // the run that holds the next share's first tile
-    if (c.t == 0 || u0 < share_begin(w, units, n_act)) continue;   // not cut, or not ours
-    const Columns co = columns_of<LIST, HT>(a, en, c);
-    if (col >= co.count) continue;
-    // parts: slot 2 w + 1, then 2 (w + 1), 2 (w + 2), ... while shares start inside the run
-    int parts = 1;
-    while (share_begin(w + parts, units, n_act) < u1 && w + parts < n_act) ++parts;
-    auto row_of = [&](int k) {
-      return static_cast<int64_t>(k == 0 ? 2 * w + 1 : 2 * (w + k)) * HT + col;
-    };
-    float m = -INFINITY;
-    for (int k = lane; k < parts; k += 32) m = fmaxf(m, wk.part_ml[row_of(k)].x);
-    m = warp_max(m);
-    const float safe = m == -INFINITY ? 0.f : m;
-    float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-    for (int k0 = 0; k0 < parts; k0 += 32) {
-      float f = 0.f;
-      if (k0 + lane < parts) {
-        const float2 ml = wk.part_ml[row_of(k0 + lane)];
-        f = ex2(ml.x - safe);
-        l += ml.y * f;
-      }
-      const int n = min(32, parts - k0);
-      for (int k = 0; k < n; k += 8) {
-        float4 v[8];
+  if (w >= wk.workers) return;
+  const Cut cut = wk.cut[w];
+  if (col >= cut.count || cut.parts == 0) return;
+  auto row_of = [&](int k) {
+    return static_cast<int64_t>(k == 0 ? 2 * w + 1 : 2 * (w + k)) * HT + col;
+  };
+  float m = -INFINITY;
+  for (int k = lane; k < cut.parts; k += 32) m = fmaxf(m, wk.part_ml[row_of(k)].x);
+  m = warp_max(m);
+  const float safe = m == -INFINITY ? 0.f : m;
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  for (int k0 = 0; k0 < cut.parts; k0 += 32) {
+    const int n = min(32, cut.parts - k0);
+    float f = 0.f;
+    if (lane < n) {
+      const float2 ml = wk.part_ml[row_of(k0 + lane)];
+      f = ex2(ml.x - safe);
+      l += ml.y * f;
+    }
+    for (int k = 0; k < n; k += 8) {
+      float4 v[8];
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          v[x] = k + x < n ? *reinterpret_cast<const float4*>(wk.part_o + row_of(k0 + k + x) * D +
-                                                              lane * 4)
-                           : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int x = 0; x < 8; ++x)
+        v[x] = k + x < n
+                   ? *reinterpret_cast<const float4*>(wk.part_o + row_of(k0 + k + x) * D + lane * 4)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const float c1 = __shfl_sync(0xffffffffu, f, (k + x) & 31);
-          if (k + x < n) {
-            o[0] += v[x].x * c1;
-            o[1] += v[x].y * c1;
-            o[2] += v[x].z * c1;
-            o[3] += v[x].w * c1;
-          }
+      for (int x = 0; x < 8; ++x) {
+        const float c = __shfl_sync(0xffffffffu, f, (k + x) & 31);
+        if (k + x < n) {
+          o[0] += v[x].x * c;
+          o[1] += v[x].y * c;
+          o[2] += v[x].z * c;
+          o[3] += v[x].w * c;
         }
       }
     }
-    l = warp_sum(l);
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    const int tok = LIST ? (co.row + col) / a.group : 0;
-    const int head = co.kvh * a.group + (LIST ? (co.row + col) % a.group : co.row + col);
-    *reinterpret_cast<uint2*>(a.out + (co.q0 + tok) * a.out_ld + static_cast<int64_t>(head) * D +
-                              lane * 4) =
-        make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
   }
+  l = warp_sum(l);
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const int tok = LIST ? (cut.row + col) / a.group : 0;
+  const int head = cut.kvh * a.group + (LIST ? (cut.row + col) % a.group : cut.row + col);
+  *reinterpret_cast<uint2*>(a.out + (cut.q0 + tok) * a.out_ld + static_cast<int64_t>(head) * D +
+                            lane * 4) =
+      make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
 }
 
 // Upper bound of the line's length.
@@ -697,7 +705,7 @@ static int64_t line_bound(const Args& a, bool list, int ht) {
 template <bool LIST, int NT>
 void launch(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const at::Tensor& like,
             cudaStream_t st) {
-  constexpr int HT = 8 * NT;
+  constexpr int HT = 8 * NT, STAGES = stages_of(NT), WARP_SMEM = STAGES * STAGE;
   Work wk;
   wk.entries = LIST ? a.num_tiles : a.num_seqs;
   const size_t lens = WARPS * sizeof(int) + Entries<LIST>::bytes(wk.entries);
@@ -706,26 +714,30 @@ void launch(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const a
   if (!attr) {
     C10_CUDA_CHECK(cudaFuncSetAttribute(rows_kernel<LIST, NT>,
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    C10_CUDA_CHECK(cudaFuncSetAttribute(join_kernel<LIST, NT>,
-                                        cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     attr = true;
   }
-  // two CTAs an SM while both fit (the entries' tables of a very large batch leave room for one); no
-  // more warps than the tiles there can be make shares
-  const int per_sm = 2 * (smem + 1024) <= 228 * 1024 ? 2 : 1;
+  // fewer CTAs an SM when the entries' tables of a very large batch need the room; no more warps
+  // than the tiles there can be make shares
+  const int per_sm = std::max<int>(1, std::min<size_t>(ctas_of(NT), 228 * 1024 / (smem + 1024)));
   const int64_t tiles = line_bound(a, LIST, HT);
   const int grid = static_cast<int>(
       std::max<int64_t>(1, std::min<int64_t>(148 * per_sm, (tiles + MIN_TILES - 1) / MIN_TILES)));
   wk.workers = grid * WARPS;
-  at::Tensor ws = at::empty({static_cast<int64_t>(wk.workers) * 2 * HT * (D + 2)},
+  static_assert(sizeof(Cut) % 8 == 0, "the partials follow the cuts");
+  const int64_t part_rows = static_cast<int64_t>(wk.workers) * 2 * HT;
+  at::Tensor ws = at::empty({wk.workers * static_cast<int64_t>(sizeof(Cut) / 4) + part_rows * (D + 2)},
                             like.options().dtype(at::kFloat));
   wk.part_o = ws.data_ptr<float>();
-  wk.part_ml = reinterpret_cast<float2*>(wk.part_o + static_cast<int64_t>(wk.workers) * 2 * HT * D);
+  wk.part_ml = reinterpret_cast<float2*>(wk.part_o + part_rows * D);
+  wk.cut = reinterpret_cast<Cut*>(wk.part_ml + part_rows);
   auto rk = rows_kernel<LIST, NT>;
   auto jk = join_kernel<LIST, NT>;
-  C10_CUDA_CHECK(launch_k(rk, dim3(grid), dim3(THREADS), smem, st, nullptr, 0, tk, tv, a, wk));
-  const int jgrid = std::min(wk.workers * HT / WARPS, 148 * 8);
-  C10_CUDA_CHECK(launch_k(jk, dim3(std::max(1, jgrid)), dim3(THREADS), lens, st, nullptr, 0, a, wk));
+  // A plain launch, after the previous kernel has left every SM: started early (programmatic
+  // launch), CTAs fill the SMs around the previous kernel's last ones unevenly, and with equal shares
+  // the fullest SM decides (256 x 2304: 163 us against 125).
+  rk<<<grid, THREADS, smem, st>>>(tk, tv, a, wk);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  C10_CUDA_CHECK(launch_k(jk, dim3(wk.workers * HT / WARPS), dim3(THREADS), 0, st, nullptr, 0, a, wk));
 }
 
 }  // namespace fp8d
