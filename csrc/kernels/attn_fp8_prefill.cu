@@ -9,7 +9,13 @@
 //
 //   warp 0      TMA: the 8-bit K and V tiles, 16-key slices, lane i slice i, into two staging
 //               buffers (K, V, K, V, ...).
-//   warp 1      MMA issuer (one thread) and TMEM owner:  O_t += P_t V_{j-1}, S_t = Q_t K_j^T.
+//   warp 1      MMA issuer and TMEM owner.  The two query tiles share one S region: a tile's softmax
+//               holds S in registers soon after it is written, and the region goes to the other tile.
+//               With slots (tile 0, 0), (tile 1, 0), (tile 0, 1), ... the issue order is S(s),
+//               O += P(s - 2) V: a softmax that ends finds its next S written, its P V runs under it,
+//               and the two softmax groups settle half a period apart, one in its exponentials while
+//               the other loads and compares.  P has columns of its own, so no MMA writes what
+//               another (of another shape, whose order is not defined) may still read.
 //   warp 2      the slices' scales of a tile, four tiles ahead.
 //   warps 4-7   convert staged codes to f16 tiles in the MMA's swizzled layout.  The codes go in
 //               unscaled: e4m3 is exact in f16, so the conversion is one cvt per pair, and rows past
@@ -20,11 +26,11 @@
 //                 P = 2^(s + log2 vs - m' + 7),  m' >= max(s + log2 vs) - 8,
 //               so P is at most 2^15 and keeps f16's 11 bits down to 2^-21 of the largest
 //               contribution; l sums P / vs in fp32.  m' moves only when the maximum passes it by 2^8
-//               (then O is rescaled in TMEM).
-// P (f16) overwrites S in TMEM and is the MMA's A operand; V is read in its key-major layout.
-// TMEM: O_t at 128 t, S_t at 256 + 128 t.  Registers: 512 threads start with 128 each and the
-// softmax warps take 200 (40 + 72 + 200 + 200 = 4 * 128 per quarter).  Every wait is bounded; on
-// expiry the kernel records an error and unwinds.
+//               (then O is rescaled in TMEM, after the previous tile's P V).
+// P (f16, in TMEM) is the MMA's A operand; V is read in its key-major layout.  TMEM: O_t at 128 t, S at
+// 256, P_t at 384 + 64 t.  Registers: 512 threads start with 128 each; the softmax warps take 200
+// (40 + 72 + 200 + 200 = 4 * 128 per quarter).  Every wait is bounded; on expiry the kernel records an
+// error and unwinds.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 
@@ -67,6 +73,47 @@ __device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t saddr, uint32_t 
 constexpr uint32_t idesc_f16(int M, int N, int b_mn_major) {
   return (1u << 4) | (static_cast<uint32_t>(b_mn_major) << 16) |
          (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
+}
+// MMAs and commits of the elected lane of a converged warp (the forms of common.cuh are for code
+// that a single lane runs).
+__device__ __forceinline__ void mma_ss_if(uint32_t leader, uint32_t d_tmem, uint64_t a_desc,
+                                          uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts_if(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem,
+                                          uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          smem_u32(bar)),
+      "r"(leader)
+      : "memory");
 }
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -124,13 +171,14 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* v_empty = v_full + VST;        // [VST] P V of every query tile done
   uint64_t* c_full = v_empty + VST;        // [CST] slice constants
   uint64_t* c_empty = c_full + CST;        // [CST] read by the 8 softmax warps
-  uint64_t* s_full = c_empty + CST;        // [QT] S_t of the key tile (and all earlier MMAs)
-  uint64_t* p_ready = s_full + QT;         // [QT] P_t in TMEM (4 softmax warps)
-  uint64_t* o_full = p_ready + QT;         // last P V done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+  uint64_t* s_full = c_empty + CST;        // [QT] S of a tile's slot (and all earlier MMAs)
+  uint64_t* s_free = s_full + QT;          // S of a slot in registers (4 softmax warps)
+  uint64_t* p_ready = s_free + 1;          // [QT] P_t in TMEM (4 softmax warps)
+  uint64_t* pv_done = p_ready + QT;        // [QT] P_t V
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + QT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kvh = blockIdx.y;
 
   if (threadIdx.x == 0) {
@@ -151,11 +199,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&c_full[s], 1);
       mbar_init(&c_empty[s], 8);
     }
+    mbar_init(s_free, 4);
     for (int t = 0; t < QT; ++t) {
       mbar_init(&s_full[t], 1);
       mbar_init(&p_ready[t], 4);
+      mbar_init(&pv_done[t], 1);
     }
-    mbar_init(o_full, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -234,55 +283,56 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) record_error(a.err, kErrTimeoutSmemEmpty);
         *abort_flag = 1;
       }
-    } else if (warp == 1 && lane == 0 && ntiles > 0) {
+    } else if (warp == 1 && ntiles > 0) {
       constexpr uint32_t idesc_s = idesc_f16(128, BN, 0);
       constexpr uint32_t idesc_o = idesc_f16(128, D, 1);
-      bool ok = mbar_wait(q_full, 0, abort_flag);
-      auto issue_pv = [&](int t, int j) {
-        if (!mbar_wait(&p_ready[t], j & 1, abort_flag)) return false;
-        tc_fence_after();
-        const uint32_t vb = smem_u32(sV(j % VST));
-        const uint32_t pc = tmem_base + 256 + 128 * t;
-#pragma unroll
-        for (int k = 0; k < BN / 16; ++k)
-          tc_mma_f16_ts(tmem_base + 128 * t, pc + k * 8,
-                        sw128_mnmajor_desc(vb + k * 16 * 128, HALF), idesc_o,
-                        (j > 0 || k > 0) ? 1u : 0u);
-        return true;
+      const uint32_t colS = tmem_base + 256;
+      static_assert(KST == 2 && VST == 2, "parities below");
+      const uint32_t leader = elect_one();
+      const uint64_t q_desc = sw128_kmajor_desc(smem_u32(sQ(0)));
+      const uint64_t k_desc = sw128_kmajor_desc(smem_u32(sK(0)));
+      const uint64_t v_desc = sw128_mnmajor_desc(smem_u32(sV(0)), HALF);
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
       };
-      auto issue_s = [&](int t, int j) {
-        const uint32_t qb = smem_u32(sQ(t)), kb = smem_u32(sK(j % KST));
-        const uint32_t sc = tmem_base + 256 + 128 * t;
+      auto issue_s = [&](int s) {
+        const int t = nqt == 2 ? s & 1 : 0, j = nqt == 2 ? s >> 1 : s;
+        if (t == 0 && !wait(&k_full[j & 1], (j >> 1) & 1)) return false;
+        if (s > 0 && !wait(s_free, (s - 1) & 1)) return false;
+        tc_fence_after();
+        const uint64_t qd = q_desc + ((t * TILE) >> 4), kd = k_desc + (((j & 1) * TILE) >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * HALF + (k & 3) * 32;
-          tc_mma_f16(sc, sw128_kmajor_desc(qb + off), sw128_kmajor_desc(kb + off), idesc_s,
-                     k > 0 ? 1u : 0u);
+          const uint32_t off = ((k >> 2) * HALF + (k & 3) * 32) >> 4;
+          mma_ss_if(leader, colS, qd + off, kd + off, idesc_s, k > 0 ? 1u : 0u);
         }
-        tc_commit(&s_full[t]);   // arrives once this and every earlier MMA have completed
+        commit_if(leader, &s_full[t]);   // arrives once this and every earlier MMA are done
+        if (t == nqt - 1) commit_if(leader, &k_empty[j & 1]);
+        return true;
       };
-      for (int j = 0; ok && j < ntiles; ++j) {
-        ok = mbar_wait(&k_full[j % KST], (j / KST) & 1, abort_flag);
-        if (ok && j > 0) ok = mbar_wait(&v_full[(j - 1) % VST], ((j - 1) / VST) & 1, abort_flag);
-        if (!ok) break;
+      auto issue_pv = [&](int s) {
+        const int t = nqt == 2 ? s & 1 : 0, j = nqt == 2 ? s >> 1 : s;
+        if (t == 0 && !wait(&v_full[j & 1], (j >> 1) & 1)) return false;
+        if (!wait(&p_ready[t], j & 1)) return false;
         tc_fence_after();
-        for (int t = 0; t < nqt && ok; ++t) {
-          if (j > 0) ok = issue_pv(t, j - 1);   // S_t is written over P_t, in issue order
-          if (ok) issue_s(t, j);
-        }
-        if (!ok) break;
-        tc_commit(&k_empty[j % KST]);
-        if (j > 0) tc_commit(&v_empty[(j - 1) % VST]);
+        const uint64_t vd = v_desc + (((j & 1) * TILE) >> 4);
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k)
+          mma_ts_if(leader, tmem_base + 128 * t, tmem_base + 384 + 64 * t + k * 8,
+                    vd + ((k * 16 * 128) >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+        if (t == nqt - 1) commit_if(leader, &v_empty[j & 1]);
+        commit_if(leader, &pv_done[t]);
+        return true;
+      };
+      const int slots = nqt * ntiles;
+      bool ok = wait(q_full, 0);
+      for (int s = 0; ok && s < slots; ++s) {
+        ok = issue_s(s);
+        if (ok && s >= nqt) ok = issue_pv(s - nqt);
       }
-      if (ok) ok = mbar_wait(&v_full[(ntiles - 1) % VST], ((ntiles - 1) / VST) & 1, abort_flag);
-      if (ok) {
-        tc_fence_after();
-        for (int t = 0; t < nqt && ok; ++t) ok = issue_pv(t, ntiles - 1);
-      }
-      if (ok) {
-        tc_commit(o_full);
-      } else {
-        record_error(a.err, kErrTimeoutTmaFull);
+      for (int s = slots - nqt; ok && s < slots; ++s) ok = issue_pv(s);
+      if (!ok) {
+        if (lane == 0) record_error(a.err, kErrTimeoutTmaFull);
         *abort_flag = 1;
       }
     } else if (warp == 2 && ntiles > 0) {
@@ -343,8 +393,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int r = 0; r < BN / 16; ++r)
         raw[r] = *reinterpret_cast<const uint4*>(src + (r * 16 + (ct >> 3)) * D +
                                                  ((c ^ ((ct >> 3) & 7)) << 4));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&st_empty[s]);
 #pragma unroll
       for (int r = 0; r < BN / 16; ++r) {
         const int row = r * 16 + (ct >> 3);
@@ -361,9 +409,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         *reinterpret_cast<uint4*>(dst + row * 128 + ((first ^ (row & 7)) << 4)) = half ? hi : lo;
         *reinterpret_cast<uint4*>(dst + row * 128 + (((first ^ 1) ^ (row & 7)) << 4)) = half ? lo : hi;
       }
+      // The staging buffer is given back only here, when every loaded code has been used: an arrival
+      // placed right behind the loads let TMA's next tile overtake some of them.
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(dst_full);
+      if (lane == 0) {
+        mbar_arrive(&st_empty[s]);
+        mbar_arrive(dst_full);
+      }
     }
     if (!ok) {
       if (lane == 0) record_error(a.err, kErrTimeoutTmaFull);
@@ -418,83 +471,92 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (lane == 0) mbar_arrive(q_full);
 
     const uint32_t tl = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t colO = 128 * t, colS = 256 + 128 * t;
+    const uint32_t colO = 128 * t, colS = 256, colP = 384 + 64 * t;
     float m_used = -INFINITY, l = 0.f, vs0 = 0.f;
     bool ok = true;
-    for (int j = 0; j < ntiles; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&c_full[j % CST], (j / CST) & 1, abort_flag));
-      if (ok && t < nqt) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, abort_flag));
-      if (!ok) {
-        if (lane == 0) record_error(a.err, kErrTimeoutTmemFull);
-        *abort_flag = 1;
-        break;
+    if (t >= nqt) {
+      // no rows in this tile: only take part in the constants' ring
+      for (int j = 0; j < ntiles && ok; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&c_full[j % CST], (j / CST) & 1, abort_flag));
+        if (ok && lane == 0) mbar_arrive(&c_empty[j % CST]);
       }
-      if (t >= nqt) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&c_empty[j % CST]);
-        continue;
-      }
+    }
+    // tiles that every row of the warp sees whole need no mask
+    const int clear = __reduce_min_sync(0xffffffffu, klim) / BN;
+    for (int j = 0; j < ntiles && t < nqt; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&c_full[j % CST], (j / CST) & 1, abort_flag) &&
+                                       mbar_wait(&s_full[t], j & 1, abort_flag));
+      if (!ok) break;
       tc_fence_after();
-      uint32_t sr[128];
+      uint32_t sr[BN];
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         tmem_ld32(tl + colS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sr + 32 * c));
-      float sc[NSL], lv[NSL], iv[NSL];
+      float sc[NSL], lv[NSL];
+      const float4* cst = sC + (j % CST) * NSL;
 #pragma unroll
       for (int i = 0; i < NSL; ++i) {
-        const float4 v = sC[(j % CST) * NSL + i];
+        const float4 v = cst[i];
         sc[i] = v.x * row_scale;
         lv[i] = v.y;
-        iv[i] = v.z;
         vs0 = v.w;
       }
       tc_wait_ld();
-      const int nvalid = min(BN, max(0, klim - j * BN));
-      if (!__all_sync(0xffffffffu, nvalid >= BN)) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free);
+      if (j >= clear) {
+        const int nvalid = min(BN, max(0, klim - j * BN));
 #pragma unroll
-        for (int c = 0; c < 128; ++c)
+        for (int c = 0; c < BN; ++c)
           if (c >= nvalid) sr[c] = __float_as_uint(-INFINITY);
       }
       // ks > 0 keeps a slice's order: maximum of the raw scores first, then its scale
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < NSL; ++i) {
-        float mg = __uint_as_float(sr[16 * i]), mh = __uint_as_float(sr[16 * i + 1]);
+        float x = __uint_as_float(sr[16 * i]), y = __uint_as_float(sr[16 * i + 1]);
 #pragma unroll
         for (int c = 2; c < 16; c += 4) {
-          mg = max3f(mg, __uint_as_float(sr[16 * i + c]), __uint_as_float(sr[16 * i + c + 1]));
+          x = max3f(x, __uint_as_float(sr[16 * i + c]), __uint_as_float(sr[16 * i + c + 1]));
           if (c + 2 < 16)
-            mh = max3f(mh, __uint_as_float(sr[16 * i + c + 2]), __uint_as_float(sr[16 * i + c + 3]));
+            y = max3f(y, __uint_as_float(sr[16 * i + c + 2]), __uint_as_float(sr[16 * i + c + 3]));
         }
-        mx = fmaxf(mx, fmaf(fmaxf(mg, mh), sc[i], lv[i]));
+        mx = fmaxf(mx, fmaf(fmaxf(x, y), sc[i], lv[i]));
+      }
+      // the previous P V has read P and is in O (it was issued when that P was ready, a softmax ago)
+      if (j > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (j - 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
       }
       const bool need = mx > m_used + LAZY;
-      const float m_new = need ? mx : m_used;
-      if (__any_sync(0xffffffffu, need) && j > 0) {
+      if (__any_sync(0xffffffffu, need)) {
+        const float m_new = need ? mx : m_used;
         const float corr = need ? ex2(m_used - m_new) : 1.f;
+        if (j > 0) {
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t ov[32];
-          tmem_ld32(tl + colO + 32 * c, ov);
-          tc_wait_ld();
+          for (int c = 0; c < 4; ++c) {
+            uint32_t ov[32];
+            tmem_ld32(tl + colO + 32 * c, ov);
+            tc_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * corr);
-          tmem_st16(tl + colO + 32 * c, *reinterpret_cast<uint32_t(*)[16]>(ov));
-          tmem_st16(tl + colO + 32 * c + 16, *reinterpret_cast<uint32_t(*)[16]>(ov + 16));
+            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * corr);
+            tmem_st16(tl + colO + 32 * c, *reinterpret_cast<uint32_t(*)[16]>(ov));
+            tmem_st16(tl + colO + 32 * c + 16, *reinterpret_cast<uint32_t(*)[16]>(ov + 16));
+          }
         }
-      }
-      if (need) {
-        l *= ex2(m_used - m_new);
+        l *= corr;
         m_used = m_new;
       }
-      const float ms = m_used == -INFINITY ? 0.f : m_used;
+      const float ms = SHIFT - (m_used == -INFINITY ? 0.f : m_used);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         uint32_t pk[16];
 #pragma unroll
         for (int i2 = 0; i2 < 2; ++i2) {
           const int i = 2 * q + i2;
-          const float add = lv[i] + (SHIFT - ms);
+          const float add = lv[i] + ms;
           const uint64_t sc2 = pack_f2(sc[i], sc[i]), ad2 = pack_f2(add, add);
           uint64_t l2 = pack_f2(0.f, 0.f);
 #pragma unroll
@@ -509,9 +571,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           float la, lb;
           unpack_f2(l2, la, lb);
-          l = fmaf(la + lb, iv[i], l);
+          l = fmaf(la + lb, cst[i].z, l);
         }
-        tmem_st16(tl + colS + 16 * q, pk);
+        tmem_st16(tl + colP + 16 * q, pk);
       }
       tc_wait_st();
       tc_fence_before();
@@ -521,9 +583,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         mbar_arrive(&c_empty[j % CST]);
       }
     }
+    if (!ok) {
+      if (lane == 0) record_error(a.err, kErrTimeoutTmemFull);
+      *abort_flag = 1;
+    }
     // ---- epilogue: O_t / l -> out[token][head][:]; rows that saw no key give 0 ----
     if (ok && t < nqt && ntiles > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(o_full, 0, abort_flag));
+      ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (ntiles - 1) & 1, abort_flag));
       if (!ok) {
         if (lane == 0) record_error(a.err, kErrTimeoutTmemFull);
         *abort_flag = 1;
