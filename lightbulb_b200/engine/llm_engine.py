@@ -29,7 +29,7 @@ import torch
 
 from ..config import CacheConfig, EngineConfig, ModelConfig, SchedulerConfig
 from ..kv.block_manager import BlockManager
-from ..models.llama import KVCache, LlamaModel
+from ..models.llama import KVCache, LlamaModel, kv_dtype_of
 from .model_runner import ModelRunner
 from .sampling import SamplingParams
 from .scheduler import Scheduler
@@ -101,7 +101,7 @@ def derive_num_blocks(cfg: ModelConfig, cache: CacheConfig, tp_size: int, device
         return cache.num_blocks
     hkv = max(1, cfg.num_kv_heads // tp_size)
     per_block = KVCache.bytes_per_block(cfg.num_layers, hkv, cache.block_size,
-                                         cfg.head_dim_padded)
+                                         cfg.head_dim_padded, kv_dtype_of(cache.kv_dtype).itemsize)
     if torch.device(device).type != "cuda":
         return max(64, (512 << 20) // per_block)
     free, _total = torch.cuda.mem_get_info(torch.device(device))
@@ -138,7 +138,7 @@ class LLMEngine:
         if comm is not None and comm.world > 1:
             nb = comm.min_int(nb)  # every rank must admit identically
         self.kv = KVCache(mcfg.num_layers, nb, self.model.hkv, cfg.cache.block_size,
-                          mcfg.head_dim_padded, device=dev)
+                          mcfg.head_dim_padded, dtype=kv_dtype_of(cfg.cache.kv_dtype), device=dev)
         self.blocks = BlockManager(nb, cfg.cache.block_size, cfg.cache.enable_prefix_caching)
         self.scheduler = Scheduler(cfg.scheduler, self.blocks)
         self.runner = ModelRunner(self.model, self.kv, self.blocks, cfg.scheduler.max_num_seqs,
@@ -155,7 +155,7 @@ class LLMEngine:
         self.overlap = bool(getattr(cfg, "overlap_decode", True))
         self._pending: Optional[_PendingStep] = None
         log.info("engine ready: %d KV blocks of %d tokens (%.1f GiB)", nb, cfg.cache.block_size,
-                 self.kv.storage.numel() * 2 / 2**30)
+                 self.kv.storage.numel() * self.kv.storage.element_size() / 2**30)
         if cfg.cache.h2o_budget > 0:
             self.enable_kv_compression("h2o", cfg.cache.h2o_budget, cfg.cache.sink_tokens,
                                        decay=cfg.cache.h2o_decay)
@@ -399,6 +399,7 @@ class LLMEngine:
                               **kw):
         """H2O heavy hitters (budget + sinks tokens kept) or StreamingLLM (sinks + window)."""
         from ..kv.compression import H2OPolicy, StreamingPolicy
+        self.kv.require_rows("KV compression")
         if kind == "h2o":
             self.kv_policy = H2OPolicy(self, budget=budget, sinks=sinks, **kw)
         elif kind == "streaming":
@@ -414,6 +415,7 @@ class LLMEngine:
         eviction under context pressure with demotion to RAM / disk and a knowledge-base fact
         per demoted span, and ``<RETRIEVE:key>`` promotion.  Replaces any other KV policy."""
         from ..kv.spans import SegmentedPolicy
+        self.kv.require_rows("the segmented cache")
         self.kv_policy = SegmentedPolicy(self, config, context_limit, segment_tokens,
                                          knowledge_base)
         return self.kv_policy

@@ -10,7 +10,10 @@ decode (``src/model_fuel/mod.rs:39-63``):
   transfer; floats and seeds take one more each; the sampled ids come back in one D2H copy;
 * decode-only steps replay a CUDA graph captured per batch-size bucket (static input
   buffers, fixed GEMM tile plans and split-KV factor); mixed prefill/decode steps run eager;
-* sampling runs on the device for all rows of the step.
+* sampling runs on the device for all rows of the step;
+* with the 8-bit KV cache the block tables stay on the device (:mod:`..kv.device_tables`): the
+  step's integers are its ids, lengths, table rows and new blocks, and ``ops.step_tables`` builds
+  positions, slots, tables and the attention work list from them.
 """
 from __future__ import annotations
 
@@ -23,6 +26,7 @@ import numpy as np
 import torch
 
 from .. import ops
+from ..kv.device_tables import ResidentTables
 from ..models.llama import ForwardBatch, KVCache, LlamaModel, prefill_tiles
 from .sampling import token_seed
 from .scheduler import ScheduledChunk, SchedulerOutput
@@ -58,11 +62,20 @@ class _GraphBucket:
         dev = r.device
         W = r.max_blocks_per_seq
         self.W = W
+        self.tables = r.tables     # 8-bit KV cache: resident block tables
+        if self.tables is not None:
+            # int32 layout: ids | ctx | new tokens | table rows | top_k | src | new blocks
+            self.n_int = 7 * bsz
+            self.ints = torch.zeros(self.n_int, dtype=torch.int32, device=dev)
+            (self.ids, self.ctx, self.q, self.rows, self.top_k, self.src,
+             self.new_blocks) = self.ints.view(7, bsz).unbind(0)
+            self.group, self.block_size = r.model.group, r.block_size
+            self._sampling(r, bsz, dev)
+            self.splits = 1
+            return
         # int32 layout: ids | pos | slots | seq_lens | cu_q(B+1) | top_k | src | block_tables(B*W)
         self.n_int = 7 * bsz + 1 + bsz * W
         self.ints = torch.zeros(self.n_int, dtype=torch.int32, device=dev)
-        self.floats = torch.zeros(2 * bsz, dtype=torch.float32, device=dev)
-        self.seeds = torch.zeros(bsz, dtype=torch.int64, device=dev)
         o = 0
 
         def take(n):
@@ -76,14 +89,25 @@ class _GraphBucket:
         self.top_k = take(bsz)
         self.src = take(bsz)           # row of the previous step whose sample feeds this row
         self.block_tables = take(bsz * W).view(bsz, W)
+        self._sampling(r, bsz, dev)
+        self.splits = ops.decode_splits(bsz, r.model.hkv, r.max_model_len) if r.is_cuda else 1
+
+    def _sampling(self, r: "ModelRunner", bsz: int, dev) -> None:
+        self.floats = torch.zeros(2 * bsz, dtype=torch.float32, device=dev)
+        self.seeds = torch.zeros(bsz, dtype=torch.int64, device=dev)
         self.temp, self.top_p = self.floats[:bsz], self.floats[bsz:]
         self.out_tokens = r.d_last_out[:bsz]   # shared by every bucket: read by the next step
         self.logits_idx = torch.arange(bsz, dtype=torch.int64, device=dev)
-        self.splits = ops.decode_splits(bsz, r.model.hkv, r.max_model_len) if r.is_cuda else 1
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.launches = 0
 
     def batch(self) -> ForwardBatch:
+        if self.tables is not None:
+            t = ops.step_tables(self.ctx, self.q, self.rows, self.tables.tables, self.new_blocks,
+                                self.bsz, self.block_size, group=self.group,
+                                num_decode=self.bsz)
+            return ForwardBatch(self.ids, t.positions, t.slots, t.block_tables, t.seq_lens,
+                                t.cu_q, self.logits_idx, num_decode=self.bsz)
         return ForwardBatch(self.ids, self.pos, self.slots, self.block_tables, self.seq_lens,
                             self.cu_q, self.logits_idx, num_decode=self.bsz,
                             decode_splits=self.splits)
@@ -113,6 +137,8 @@ class ModelRunner:
         self.block_size = kv.block_size
         self.max_blocks_per_seq = (max_model_len + self.block_size - 1) // self.block_size + 1
         self.use_graphs = use_cuda_graphs and self.is_cuda
+        self.tables = ResidentTables(max_num_seqs + 8, self.max_blocks_per_seq, self.device) \
+            if kv.fp8 else None
         step = comm.world if (comm is not None and getattr(comm, "fused_requested", False)) else 1
         # fused tensor-parallel decode needs T % world == 0: round buckets up to multiples
         bk = sorted({((b + step - 1) // step) * step for b in graph_buckets if b <= max_num_seqs})
@@ -124,7 +150,7 @@ class ModelRunner:
         self.graph_pool = None
         self.comm = comm
         pin = self.is_cuda
-        n_int = 6 * self.max_tokens + 3 * (max_num_seqs + 1) + max_num_seqs * self.max_blocks_per_seq
+        n_int = 6 * self.max_tokens + 4 * (max_num_seqs + 1) + max_num_seqs * self.max_blocks_per_seq
         # sampled rows per step: one per sequence, or every row of a verify chunk
         ns = self.max_tokens + 1
         # Two sets of pinned input buffers, alternated per launch: with overlapped decode the
@@ -264,6 +290,27 @@ class ModelRunner:
         return (self.comm is not None and self.comm.world > 1 and
                 all(c.seq.params.temperature <= 0 for c in chunks))
 
+    def _fill_graph_tables(self, hi, chunks: List[ScheduledChunk], bsz: int, W: int):
+        """Host-built integers of a decode step (bf16 KV cache): ids, positions, slots, lengths,
+        query offsets and block tables; returns the views that the caller completes."""
+        B = len(chunks)
+        ids, pos, slots = hi[:bsz], hi[bsz:2 * bsz], hi[2 * bsz:3 * bsz]
+        seq_lens, cu_q = hi[3 * bsz:4 * bsz], hi[4 * bsz:5 * bsz + 1]
+        top_k = hi[5 * bsz + 1:6 * bsz + 1]
+        src = hi[6 * bsz + 1:7 * bsz + 1]
+        bt = hi[7 * bsz + 1:].reshape(bsz, W)
+        slots[:] = -1
+        for i, c in enumerate(chunks):
+            s = c.seq
+            ids[i] = s.last_token
+            pos[i] = c.start + getattr(s, "evicted", 0)
+            slots[i] = c.slots[0]
+            seq_lens[i] = c.start + 1
+        cu_q[:B + 1] = np.arange(B + 1, dtype=np.int32)
+        cu_q[B + 1:] = B
+        self._fill_block_tables([c.seq for c in chunks], bt[:B], W)
+        return ids, top_k, src
+
     def _run_graph(self, chunks: List[ScheduledChunk], src_rows=None, defer: bool = False):
         B = len(chunks)
         bsz = self.buckets[bisect.bisect_left(self.buckets, B)]
@@ -275,26 +322,24 @@ class ModelRunner:
         self._next_host_inputs()
         hi = self.h_ints[:g.n_int].numpy()
         hi[:] = 0
-        ids, pos, slots = hi[:bsz], hi[bsz:2 * bsz], hi[2 * bsz:3 * bsz]
-        seq_lens, cu_q = hi[3 * bsz:4 * bsz], hi[4 * bsz:5 * bsz + 1]
-        top_k = hi[5 * bsz + 1:6 * bsz + 1]
-        src = hi[6 * bsz + 1:7 * bsz + 1]
-        bt = hi[7 * bsz + 1:].reshape(bsz, W)
-        slots[:] = -1
+        if g.tables is not None:
+            ids, ctx, q, rows, top_k, src, new_blocks = hi.reshape(7, bsz)
+            ctx[:B] = [c.start for c in chunks]
+            q[:B] = 1
+            ids[:B] = [c.seq.last_token for c in chunks]
+            bt = np.empty((B, W), dtype=np.int32)
+            seqs = [c.seq for c in chunks]
+            self._fill_block_tables(seqs, bt, W)
+            rows[:B], new = g.tables.place([s.seq_id for s in seqs], bt, ctx[:B], q[:B],
+                                           self.block_size)
+            new_blocks[:len(new)] = new
+        else:
+            ids, top_k, src = self._fill_graph_tables(hi, chunks, bsz, W)
         src[:] = -1
-        for i, c in enumerate(chunks):
-            s = c.seq
-            ids[i] = s.last_token
-            pos[i] = c.start + getattr(s, "evicted", 0)
-            slots[i] = c.slots[0]
-            seq_lens[i] = c.start + 1
         if src_rows is not None:
             sr = np.asarray(src_rows, dtype=np.int32)
             src[:B] = sr
             ids[:B][sr >= 0] = 0
-        cu_q[:B + 1] = np.arange(B + 1, dtype=np.int32)
-        cu_q[B + 1:] = B
-        self._fill_block_tables([c.seq for c in chunks], bt[:B], W)
         temps, tk, tp, seeds = self._sampling_rows(chunks)
         top_k[:B] = tk
         hf = self.h_floats[:2 * bsz].numpy()
@@ -318,10 +363,12 @@ class ModelRunner:
         # overlapped step launched next still has to read: keep its contents
         saved = self.d_last_out.clone()
         g = _GraphBucket(self, bsz, greedy)
-        # valid dummy inputs: every row points at block 0 with one token, no KV write
-        g.cu_q.copy_(torch.arange(bsz + 1, dtype=torch.int32))
-        g.seq_lens.fill_(1)
-        g.slots.fill_(-1)
+        if g.tables is None:
+            # valid dummy inputs: every row points at block 0 with one token, no KV write
+            g.cu_q.copy_(torch.arange(bsz + 1, dtype=torch.int32))
+            g.seq_lens.fill_(1)
+            g.slots.fill_(-1)
+        # (8-bit cache: zero lengths are valid dummies, padded rows without keys)
         g.src.fill_(-1)
         g.temp.fill_(0.0)
         s = torch.cuda.Stream()
@@ -369,14 +416,19 @@ class ModelRunner:
             o += n
             return v
 
-        ids, pos, slots = take(T), take(T), take(T)
-        seq_lens, cu_q = take(B), take(B + 1)
+        fp8 = self.tables is not None
+        ids = take(T)
+        if fp8:
+            ctx, q_lens, rows = take(B), take(B), take(B)
+            seq_lens, cu_q = np.empty(B, np.int32), np.empty(B + 1, np.int32)
+        else:
+            pos, slots = take(T), take(T)
+            seq_lens, cu_q = take(B), take(B + 1)
         nlog = sum((c.num_tokens if c.logits_all else 1) for c in chunks if c.needs_logits)
         logits_idx = take(nlog)
         top_k = take(nlog)
         src = take(num_decode)
-        bt = take(B * width).reshape(B, width)
-        n_int = o
+        bt = np.empty((B, width), np.int32) if fp8 else take(B * width).reshape(B, width)
         t = 0
         li = 0
         cu_q[0] = 0
@@ -385,8 +437,11 @@ class ModelRunner:
             n = c.num_tokens
             t0 = c.start + getattr(s, "evicted", 0)   # token index (KV index + evicted)
             ids[t:t + n] = s.all_token_ids[t0:t0 + n]
-            pos[t:t + n] = np.arange(t0, t0 + n, dtype=np.int32)
-            slots[t:t + n] = c.slots
+            if fp8:
+                ctx[i], q_lens[i] = c.start, n
+            else:
+                pos[t:t + n] = np.arange(t0, t0 + n, dtype=np.int32)
+                slots[t:t + n] = c.slots
             t += n
             seq_lens[i] = c.start + n
             cu_q[i + 1] = t
@@ -404,6 +459,13 @@ class ModelRunner:
             src[:] = sr
             ids[:num_decode][sr >= 0] = 0
         self._fill_block_tables([c.seq for c in chunks], bt, width)
+        n_new = 0
+        if fp8:
+            rows[:], new = self.tables.place([c.seq.seq_id for c in chunks], bt, ctx, q_lens,
+                                             self.block_size)
+            n_new = len(new)
+            take(n_new)[:] = new
+        n_int = o
         temps, tk, tp, seeds = self._sampling_rows(chunks)
         top_k[:] = tk
         hf = self.h_floats[:2 * max(nlog, 1)].numpy()
@@ -425,26 +487,37 @@ class ModelRunner:
             o += n
             return v
 
-        d_ids, d_pos, d_slots = dtake(T), dtake(T), dtake(T)
-        d_seq_lens, d_cu_q = dtake(B), dtake(B + 1)
+        d_ids = dtake(T)
+        if fp8:
+            d_ctx, d_q, d_rows = dtake(B), dtake(B), dtake(B)
+        else:
+            d_pos, d_slots = dtake(T), dtake(T)
+            d_seq_lens, d_cu_q = dtake(B), dtake(B + 1)
         d_logits_idx = dtake(nlog).long()
         d_top_k = dtake(nlog)
         d_src = dtake(num_decode)
-        d_bt = dtake(B * width).view(B, width)
+        if fp8:
+            st = ops.step_tables(d_ctx, d_q, d_rows, self.tables.tables, dtake(n_new), T,
+                                 self.block_size, group=self.model.group, num_decode=num_decode)
+            d_pos, d_slots, d_bt = st.positions, st.slots, st.block_tables
+            d_seq_lens, d_cu_q = st.seq_lens, st.cu_q
+            tiles = (st.tile_seq, st.tile_row0) if num_decode < B else None
+        else:
+            d_bt = dtake(B * width).view(B, width)
+            cu_list = cu_q.tolist()
+            ts, tr = prefill_tiles(cu_list, num_decode, self.model.group,
+                                   block_size=self.block_size, head_dim=self.model.d)
+            tiles = torch.tensor([ts, tr], dtype=torch.int32).to(self.device, non_blocking=True) \
+                if ts else None
         if fwd:
             ops.forward_tokens(d_ids[:num_decode], d_src, self.d_last_out)
-        cu_list = cu_q.tolist()
-        ts, tr = prefill_tiles(cu_list, num_decode, self.model.group,
-                               block_size=self.block_size, head_dim=self.model.d)
-        tiles = torch.tensor([ts, tr], dtype=torch.int32).to(self.device, non_blocking=True) \
-            if ts else None
         max_len = int(seq_lens.max()) if B else 1
         fb = ForwardBatch(d_ids, d_pos, d_slots, d_bt, d_seq_lens, d_cu_q, d_logits_idx,
                           num_decode=num_decode,
                           tile_seq=tiles[0] if tiles is not None else None,
                           tile_row0=tiles[1] if tiles is not None else None,
                           decode_splits=ops.decode_splits(num_decode, self.model.hkv, max_len)
-                          if self.is_cuda else 1,
+                          if self.is_cuda and not fp8 else 1,
                           seq_lens_cpu=torch.from_numpy(seq_lens.copy()),
                           cu_q_cpu=torch.from_numpy(cu_q.copy()))
         ev = self._ev_start() if self.is_cuda else None

@@ -107,6 +107,8 @@ def save_engine_state(engine, path: str, request_ids=None, include_kv: bool = Tr
     returned in ``["drained"]`` so the caller can still deliver them."""
     import dataclasses
     from ..kv.tiers import encode_tensors
+    if include_kv:
+        engine.kv.require_rows("saving KV rows (include_kv)")
     drained = engine.drain()
     reqs, tensors = [], {}
     for rid, s in engine.seqs.items():
@@ -152,6 +154,8 @@ def restore_engine_state(engine, path: str) -> List[str]:
                                                                  st.shape[5]):
         raise ValueError(f"snapshot of a different model shape: {meta['layers']} layers, "
                          f"{meta['kv_heads']} KV heads, head dim {meta['head_dim']}")
+    if any(r["num_cached"] for r in meta["requests"]):
+        engine.kv.require_rows("restoring KV rows")
     engine.drain()
     bm, sch = engine.blocks, engine.scheduler
     bs = st.shape[4]

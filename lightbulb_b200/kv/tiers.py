@@ -182,6 +182,8 @@ class BlockTierMover:
 
     def __init__(self, engine, disk: Optional[DiskStore] = None, max_ram_entries: int = 64,
                  knowledge_base=None, summarize=None):
+        if getattr(getattr(engine, "kv", None), "fp8", False):
+            engine.kv.require_rows("tiered storage")
         self.eng = engine
         self.disk = disk
         self.max_ram = max_ram_entries

@@ -27,8 +27,20 @@ from .. import ops
 from ..config import ModelConfig
 
 
+KV_DTYPES = {"bf16": torch.bfloat16, "fp8": ops.FP8_KV_DTYPE}
+
+
+def kv_dtype_of(name: str) -> torch.dtype:
+    """Element type of ``CacheConfig.kv_dtype``."""
+    if name not in KV_DTYPES:
+        raise ValueError(f"kv_dtype {name!r}: one of {sorted(KV_DTYPES)}")
+    return KV_DTYPES[name]
+
+
 class KVCache:
-    """Paged KV storage: per layer K and V tensors of shape [num_blocks, Hkv, BS, D]."""
+    """Paged KV storage: per layer K and V tensors of shape [num_blocks, Hkv, BS, D].  With the
+    8-bit element type (``kv_dtype="fp8"``) also one fp32 scale per block and KV head,
+    ``k_scale`` / ``v_scale`` [num_blocks, Hkv] per layer."""
 
     def __init__(self, num_layers: int, num_blocks: int, num_kv_heads: int, block_size: int,
                  head_dim: int, dtype=torch.bfloat16, device="cuda"):
@@ -37,14 +49,31 @@ class KVCache:
         self.block_size = block_size
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
-        self.storage = torch.zeros(num_layers, 2, num_blocks, num_kv_heads, block_size, head_dim,
-                                   dtype=dtype, device=device)
+        self.fp8 = dtype == ops.FP8_KV_DTYPE
+        if self.fp8 and (block_size not in (16, 32, 64) or head_dim != 128):
+            raise ValueError(f"fp8 KV cache: block size 16, 32 or 64 and 128-wide heads "
+                             f"(got {block_size}, {head_dim})")
+        shape = (num_layers, 2, num_blocks, num_kv_heads, block_size, head_dim)
+        if self.fp8:
+            self.storage = torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype)
+            self.scales = torch.ones(shape[:4], device=device)
+            self.k_scale = [self.scales[i, 0] for i in range(num_layers)]
+            self.v_scale = [self.scales[i, 1] for i in range(num_layers)]
+        else:
+            self.storage = torch.zeros(shape, dtype=dtype, device=device)
         self.k = [self.storage[i, 0] for i in range(num_layers)]
         self.v = [self.storage[i, 1] for i in range(num_layers)]
 
     @staticmethod
     def bytes_per_block(num_layers, num_kv_heads, block_size, head_dim, elt=2) -> int:
-        return num_layers * 2 * num_kv_heads * block_size * head_dim * elt
+        """``elt``: bytes per element; 1 counts the 8-bit cache's scales too."""
+        return num_layers * 2 * num_kv_heads * (block_size * head_dim * elt +
+                                                (4 if elt == 1 else 0))
+
+    def require_rows(self, what: str) -> None:
+        """Refuse features that read or write single token rows as bf16."""
+        if self.fp8:
+            raise ValueError(f"{what} works on bf16 KV rows: not with kv_dtype='fp8'")
 
     def copy_blocks(self, pairs: List[int]) -> None:
         """Copy-on-write: pairs = [src0, dst0, src1, dst1, ...]."""
@@ -52,6 +81,11 @@ class KVCache:
             return
         src = torch.tensor(pairs[0::2], device=self.storage.device, dtype=torch.long)
         dst = torch.tensor(pairs[1::2], device=self.storage.device, dtype=torch.long)
+        if self.fp8:
+            raw = self.storage.view(torch.uint8)
+            raw[:, :, dst] = raw[:, :, src]
+            self.scales[:, :, dst] = self.scales[:, :, src]
+            return
         self.storage[:, :, dst] = self.storage[:, :, src]
 
 
@@ -145,11 +179,7 @@ class LlamaModel:
         attn = torch.empty(T, hq * d, dtype=torch.bfloat16, device=self.device)
         for i, L in enumerate(self.layers):
             qkv = F.gemm_consume(h, L["qkv"])
-            self._rope_kv(qkv, b, kv, i, L)
-            q = qkv[:, :hq * d].view(T, hq, d)
-            ops.paged_attention(q, kv.k[i], kv.v[i], b.block_tables, b.seq_lens, b.cu_q,
-                                attn.view(T, hq, d), self.group, decode=True,
-                                num_splits=b.decode_splits, scale=self.scale)
+            self._attend(qkv, b, kv, i, L, attn.view(T, hq, d))
             F.gemm_scatter(attn, L["o"], R)
             F.norm_gather(L["ln_post"], R, eps)
             act = F.gemm_consume(h, L["gate_up"], mode=ops.EPI_SWIGLU)
@@ -184,19 +214,7 @@ class LlamaModel:
         nl = len(self.layers)
         for i, L in enumerate(self.layers):
             qkv = ops.gemm(h, L["qkv"])
-            self._rope_kv(qkv, b, kv, i, L)
-            q = qkv[:, :hq * d].view(T, hq, d)
-            a3 = attn.view(T, hq, d)
-            if nd > 0:
-                ops.paged_attention(q, kv.k[i], kv.v[i], b.block_tables[:nd], b.seq_lens[:nd],
-                                    b.cu_q[:nd + 1], a3, self.group, decode=True,
-                                    num_splits=b.decode_splits, scale=self.scale,
-                                    seq_lens_cpu=b.seq_lens_cpu, cu_q_cpu=b.cu_q_cpu)
-            if b.tile_seq is not None and b.tile_seq.numel() > 0:
-                ops.paged_attention(q, kv.k[i], kv.v[i], b.block_tables, b.seq_lens, b.cu_q,
-                                    a3, self.group, decode=False, tile_seq=b.tile_seq,
-                                    tile_row0=b.tile_row0, seq_lens_cpu=b.seq_lens_cpu,
-                                    cu_q_cpu=b.cu_q_cpu, scale=self.scale)
+            q = self._attend(qkv, b, kv, i, L, attn.view(T, hq, d))
             if self.h2o is not None and nd > 0 and i == nl - 1:
                 self.h2o.accumulate(q[:nd], kv.k[i], b.block_tables[:nd], b.seq_lens[:nd])
             h = X.gemm_norm(attn, L["o"], x_own, L["ln_post"], eps)
@@ -236,19 +254,7 @@ class LlamaModel:
         nd = b.num_decode
         for i, L in enumerate(self.layers):
             qkv = ops.gemm(h, L["qkv"])
-            self._rope_kv(qkv, b, kv, i, L)
-            q = qkv[:, :hq * d].view(T, hq, d)
-            a3 = attn.view(T, hq, d)
-            if nd > 0:
-                ops.paged_attention(q, kv.k[i], kv.v[i], b.block_tables[:nd], b.seq_lens[:nd],
-                                    b.cu_q[:nd + 1], a3, self.group, decode=True,
-                                    num_splits=b.decode_splits, scale=self.scale,
-                                    seq_lens_cpu=b.seq_lens_cpu, cu_q_cpu=b.cu_q_cpu)
-            if b.tile_seq is not None and b.tile_seq.numel() > 0:
-                ops.paged_attention(q, kv.k[i], kv.v[i], b.block_tables, b.seq_lens, b.cu_q,
-                                    a3, self.group, decode=False, tile_seq=b.tile_seq,
-                                    tile_row0=b.tile_row0, seq_lens_cpu=b.seq_lens_cpu,
-                                    cu_q_cpu=b.cu_q_cpu, scale=self.scale)
+            q = self._attend(qkv, b, kv, i, L, attn.view(T, hq, d))
             if self.h2o is not None and nd > 0 and i == len(self.layers) - 1 and last:
                 self.h2o.accumulate(q[:nd], kv.k[i], b.block_tables[:nd], b.seq_lens[:nd])
             if comm is not None:
@@ -270,6 +276,40 @@ class LlamaModel:
             return x
         hl = h.index_select(0, b.logits_idx) if b.logits_idx.numel() != T else h
         return ops.gemm(hl, self.w["lm_head"], mode=ops.EPI_F32)
+
+    def _attend(self, qkv: torch.Tensor, b: ForwardBatch, kv: KVCache, i: int, L,
+                out: torch.Tensor) -> torch.Tensor:
+        """RoPE, KV append and attention of layer ``i`` into ``out`` [T, hq, D]: the decode kernel
+        for the first ``num_decode`` rows, the prefill kernel for the work list's.  Returns the
+        rotated q."""
+        T, nd = qkv.shape[0], b.num_decode
+        tiles = b.tile_seq is not None and b.tile_seq.numel() > 0
+        if kv.fp8:
+            cache = (kv.k[i], kv.v[i], kv.k_scale[i], kv.v_scale[i])
+            q = ops.rope_kv_fp8(qkv, b.positions, b.slots, self.cos_sin, *cache, self.hq, self.hkv,
+                                q_norm=L.get("q_norm"), k_norm=L.get("k_norm"),
+                                norm_dim=self.cfg.head_dim, eps=self.cfg.rms_norm_eps)
+            if nd > 0:
+                ops.paged_attention_fp8(q, *cache, b.block_tables[:nd], b.seq_lens[:nd], None, out,
+                                        self.group, decode=True, scale=self.scale)
+            if tiles:
+                ops.paged_attention_fp8(q, *cache, b.block_tables, b.seq_lens, b.cu_q, out,
+                                        self.group, decode=False, tile_seq=b.tile_seq,
+                                        tile_row0=b.tile_row0, scale=self.scale)
+            return q
+        self._rope_kv(qkv, b, kv, i, L)
+        q = qkv[:, :self.hq * self.d].view(T, self.hq, self.d)
+        if nd > 0:
+            ops.paged_attention(q, kv.k[i], kv.v[i], b.block_tables[:nd], b.seq_lens[:nd],
+                                b.cu_q[:nd + 1], out, self.group, decode=True,
+                                num_splits=b.decode_splits, scale=self.scale,
+                                seq_lens_cpu=b.seq_lens_cpu, cu_q_cpu=b.cu_q_cpu)
+        if tiles:
+            ops.paged_attention(q, kv.k[i], kv.v[i], b.block_tables, b.seq_lens, b.cu_q, out,
+                                self.group, decode=False, tile_seq=b.tile_seq,
+                                tile_row0=b.tile_row0, seq_lens_cpu=b.seq_lens_cpu,
+                                cu_q_cpu=b.cu_q_cpu, scale=self.scale)
+        return q
 
     def _rope_kv(self, qkv: torch.Tensor, b: ForwardBatch, kv: KVCache, i: int, L) -> None:
         """RoPE + paged KV append of layer ``i`` (with Qwen3's per-head q/k RMSNorm when the
