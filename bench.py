@@ -75,6 +75,8 @@ def parse():
     ap.add_argument("--h2o-budget", type=int, default=2048)
     ap.add_argument("--h2o-sinks", type=int, default=4)
     ap.add_argument("--block-size", type=int, default=16)
+    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "fp8"],
+                    help="KV cache elements of the decode config")
     ap.add_argument("--max-batched-tokens", type=int, default=16384)
     ap.add_argument("--comm", default="p2p", choices=["nccl", "fused", "p2p", "allreduce"],
                     help="TP partial-sum collective (engine option parallel.comm)")
@@ -220,7 +222,8 @@ def bench_decode(args):
     max_len = args.max_prompt + out_len + 16
     ecfg = EngineConfig(
         model=mcfg,
-        cache=CacheConfig(block_size=args.block_size, gpu_memory_utilization=0.92),
+        cache=CacheConfig(block_size=args.block_size, gpu_memory_utilization=0.92,
+                          kv_dtype=args.kv_dtype),
         scheduler=SchedulerConfig(max_num_seqs=args.requests,
                                   max_num_batched_tokens=args.max_batched_tokens,
                                   chunk_size=args.max_batched_tokens, max_model_len=max_len),
@@ -325,7 +328,9 @@ def bench_decode(args):
             "config": {"model": describe(mcfg),
                        "global_batch": args.requests, "seq_len": f"prompt U[{args.min_prompt},"
                        f"{args.max_prompt}] + {out_len} out", "parallelism": f"tp{world}",
-                       "kv_block": args.block_size, "comm": args.comm if world > 1 else "none",
+                       "kv_block": args.block_size,
+                       **({"kv_dtype": args.kv_dtype} if args.kv_dtype != "bf16" else {}),
+                       "comm": args.comm if world > 1 else "none",
                        "l2": "inputs larger than L2 (16 GB weights + KV per step)",
                        "cuda_graphs": not args.no_graphs},
             "ttft_p50_ms": round(1e3 * ttfts[len(ttfts) // 2], 2),

@@ -19,8 +19,8 @@ import sys
 
 
 def build_state(model_path, engine_overrides=None, random_model=None, comm=None, rank=0,
-                world=1, start_engine=True):
-    from ..config import EngineConfig, SchedulerConfig, ServerConfig, get_preset
+                world=1, start_engine=True, kv_dtype="bf16"):
+    from ..config import CacheConfig, EngineConfig, SchedulerConfig, ServerConfig, get_preset
     from ..engine.async_engine import AsyncEngine
     from ..engine.llm_engine import LLMEngine
     from ..server.app import AppState
@@ -31,13 +31,15 @@ def build_state(model_path, engine_overrides=None, random_model=None, comm=None,
     name = "lightbulb-default"
     if random_model:
         cfg = get_preset(random_model)
-        ecfg = EngineConfig(scheduler=SchedulerConfig(max_model_len=sc.max_context))
+        ecfg = EngineConfig(cache=CacheConfig(kv_dtype=kv_dtype),
+                            scheduler=SchedulerConfig(max_model_len=sc.max_context))
         eng = LLMEngine.random_init(cfg, ecfg, comm=comm, tp_rank=rank, tp_size=world)
         engine = AsyncEngine(eng) if start_engine else eng
         name = random_model
         template = resolve_for_model(None, eng.tokenizer)
     elif model_path and os.path.exists(model_path):
-        ecfg = EngineConfig(scheduler=SchedulerConfig(max_model_len=sc.max_context))
+        ecfg = EngineConfig(cache=CacheConfig(kv_dtype=kv_dtype),
+                            scheduler=SchedulerConfig(max_model_len=sc.max_context))
         eng = LLMEngine.from_pretrained(model_path, ecfg, comm=comm, tp_rank=rank, tp_size=world)
         engine = AsyncEngine(eng) if start_engine else eng
         template = resolve_for_model(model_path, eng.tokenizer)
@@ -52,6 +54,8 @@ def main(argv=None) -> int:
     ap.add_argument("--model", default=None)
     ap.add_argument("--random-model", default=None, help="preset name: random-init weights")
     ap.add_argument("--bind", default=None)
+    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "fp8"],
+                    help="KV cache elements; fp8 halves the cache's bytes")
     a = ap.parse_args(argv)
     logging.basicConfig(level=os.environ.get("LIGHTBULB_LOG", "INFO"))
     from ..config import ServerConfig
@@ -59,7 +63,7 @@ def main(argv=None) -> int:
     model = a.model or os.path.join(sc.models_dir, sc.default_model)
     if int(os.environ.get("WORLD_SIZE", "1")) > 1:
         return _serve_tp(a, model)
-    state, sc = build_state(model, random_model=a.random_model)
+    state, sc = build_state(model, random_model=a.random_model, kv_dtype=a.kv_dtype)
     from ..server.app import create_app
     from ..server.tls import ssl_kwargs
     import uvicorn
@@ -80,7 +84,7 @@ def _serve_tp(a, model) -> int:
     rank, world, _ = init_distributed(timeout_s=600)
     comm = TPComm()
     state, sc = build_state(model, random_model=a.random_model, comm=comm, rank=rank,
-                            world=world, start_engine=(rank == 0))
+                            world=world, start_engine=(rank == 0), kv_dtype=a.kv_dtype)
     if state.engine is None:
         raise SystemExit("tensor-parallel serving needs --model or --random-model")
     plane = ControlPlane()
