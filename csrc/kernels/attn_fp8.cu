@@ -76,7 +76,7 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
     if (B == 0) return;
     TORCH_CHECK(fp8_rows_fits(a, false), op,
                 ": at most 4096 sequences, and 2^31 / 32 keys x KV heads in their tables");
-    fp8_rows(a, false, tk, tv, q, st);
+    fp8_rows(a, false, group, tk, tv, q, st);
     return;
   }
   TORCH_CHECK(cu_q.has_value() && tile_seq.has_value() && tile_row0.has_value(), op,
@@ -91,10 +91,12 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   a.tile_row0 = tile_row0->data_ptr<int>();
   a.num_tiles = tile_seq->numel();
   // At most FEW_ROWS query rows per item on average (verification of a few tokens, tails of prompts):
-  // 256-row tiles would be mostly padding.
+  // 256-row tiles would be mostly padding.  rows / tcgen05 kernel, us: 32 rows 64 x 4000 keys 196 / 278,
+  // 32 x 1280 49 / 52; 48 rows 32 x 1280 64 / 52; 64 rows 81 / 52.
   constexpr int64_t FEW_ROWS = 32;
-  if (q.size(0) * group <= FEW_ROWS * a.num_tiles && fp8_rows_fits(a, true))
-    fp8_rows(a, true, tk, tv, q, st);
+  const int64_t avg = (q.size(0) * group + a.num_tiles - 1) / a.num_tiles;
+  if (avg <= FEW_ROWS && fp8_rows_fits(a, true))
+    fp8_rows(a, true, avg, tk, tv, q, st);
   else
     fp8_prefill(a, tk, tv, st);
 }

@@ -44,10 +44,12 @@ constexpr int KT = 32;                        // keys per tile
 constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
 constexpr int STAGE = 2 * 2 * SLICE;          // K slices, then V slices
-// One column tile: 2 stages and 12 warps an SM; two: 3 stages and 8 warps (their O takes twice the
-// registers).  Both keep 192 KB of an SM in flight.
-constexpr int stages_of(int nt) { return nt == 1 ? 2 : 3; }
+// One column tile of 8: 2 stages and 12 warps an SM; two: 3 stages and 8 warps (their O takes twice
+// the registers): 192 KB of an SM in flight.  Three: 2 stages, and q's fragments wait in shared
+// memory, each lane's own, instead of 48 registers.
+constexpr int stages_of(int nt) { return nt == 2 ? 3 : 2; }
 constexpr int ctas_of(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int q_smem_of(int nt) { return nt > 2 ? nt * 8 * 32 * 8 : 0; }    // bytes per warp
 constexpr int MAX_ENTRIES = 4096;
 constexpr int ENTRY_ROWS = 256;               // packed query rows of a work list's item
 constexpr int MIN_TILES = 4;                  // per share: less is not worth a partial result
@@ -269,11 +271,14 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
                                              ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ring = smem + warp * WARP_SMEM;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + WARPS * WARP_SMEM) + warp * STAGES;
+  constexpr bool Q_SMEM = q_smem_of(NT) > 0;
+  constexpr int META = WARPS * (WARP_SMEM + q_smem_of(NT));
+  uint2* s_q = reinterpret_cast<uint2*>(smem + WARPS * WARP_SMEM + warp * q_smem_of(NT)) + lane;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + META) + warp * STAGES;
   // scales of a stage's slices: [stage][slice][ks, vs]
-  float* s_scale = reinterpret_cast<float*>(smem + WARPS * WARP_SMEM + WARPS * STAGES * 8) +
+  float* s_scale = reinterpret_cast<float*>(smem + META + WARPS * STAGES * 8) +
                    warp * STAGES * 4;
-  int* s_tot = reinterpret_cast<int*>(smem + WARPS * WARP_SMEM + WARPS * STAGES * 24);
+  int* s_tot = reinterpret_cast<int*>(smem + META + WARPS * STAGES * 24);
   const Entries<LIST> en(s_tot + WARPS, wk.entries);
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 3);   // lane 0's expect + two scale loads
@@ -375,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
     // ---- tiles [t0, t1) of one run ----
     const int t0 = cc.t, t1 = min(cc.nt, t0 + u_end - u), len = en.lim[cc.e];
     const Columns co = columns_of<LIST, HT>(a, en, cc);
-    uint32_t qf[NT][8][2];
+    uint32_t qf[Q_SMEM ? 1 : NT][8][2];
     float hs[NT][2];
     // where column i's row lies in q and out, and the keys that it sees
     auto token_of = [&](int i) { return LIST ? (co.row + i) / a.group : 0; };
@@ -413,8 +418,13 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
       for (int c = 0; c < 8; ++c) {
         const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[c].x));
         const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[c].y));
-        qf[n][c][0] = pack_f16x2(x.x * up, x.y * up);
-        qf[n][c][1] = pack_f16x2(y.x * up, y.y * up);
+        const uint2 f = make_uint2(pack_f16x2(x.x * up, x.y * up), pack_f16x2(y.x * up, y.y * up));
+        if (Q_SMEM) {
+          s_q[(n * 8 + c) * 32] = f;
+        } else {
+          qf[Q_SMEM ? 0 : n][c][0] = f.x;
+          qf[Q_SMEM ? 0 : n][c][1] = f.y;
+        }
       }
       const float down = pow2i(-sh) * a.scale_log2;
       hs[n][0] = __shfl_sync(0xffffffffu, down, t4 * 8);
@@ -460,8 +470,16 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
           e4m3x4_to_f16(r[3], y[1], y[3]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            mma_f16(s[i][n], x[0], x[1], x[2], x[3], qf[n][c][0], qf[n][c][1]);
-            mma_f16(s[i][n], y[0], y[1], y[2], y[3], qf[n][c + 1][0], qf[n][c + 1][1]);
+            uint2 f, h;
+            if (Q_SMEM) {
+              f = s_q[(n * 8 + c) * 32];
+              h = s_q[(n * 8 + c + 1) * 32];
+            } else {
+              f = make_uint2(qf[Q_SMEM ? 0 : n][c][0], qf[Q_SMEM ? 0 : n][c][1]);
+              h = make_uint2(qf[Q_SMEM ? 0 : n][c + 1][0], qf[Q_SMEM ? 0 : n][c + 1][1]);
+            }
+            mma_f16(s[i][n], x[0], x[1], x[2], x[3], f.x, f.y);
+            mma_f16(s[i][n], y[0], y[1], y[2], y[3], h.x, h.y);
           }
         }
         const float ks = i ? sc1.x : sc0.x;
@@ -709,7 +727,7 @@ void launch(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const a
   Work wk;
   wk.entries = LIST ? a.num_tiles : a.num_seqs;
   const size_t lens = WARPS * sizeof(int) + Entries<LIST>::bytes(wk.entries);
-  const size_t smem = 1024 + WARPS * WARP_SMEM + WARPS * STAGES * 24 + lens;
+  const size_t smem = 1024 + WARPS * (WARP_SMEM + q_smem_of(NT)) + WARPS * STAGES * 24 + lens;
   static bool attr = false;
   if (!attr) {
     C10_CUDA_CHECK(cudaFuncSetAttribute(rows_kernel<LIST, NT>,
@@ -747,12 +765,16 @@ bool fp8_rows_fits(const fp8a::Args& a, bool list) {
          fp8d::line_bound(a, list, 8) < (int64_t(1) << 31);
 }
 
-void fp8_rows(const fp8a::Args& a, bool list, const CUtensorMap& tk, const CUtensorMap& tv,
-              const at::Tensor& like, cudaStream_t st) {
+void fp8_rows(const fp8a::Args& a, bool list, int64_t rows, const CUtensorMap& tk,
+              const CUtensorMap& tv, const at::Tensor& like, cudaStream_t st) {
   using namespace fp8d;
-  // decode: a group of up to 8 heads fills one column tile; a list's rows are (token, head) pairs,
-  // usually more than 8
-  if (list) launch<true, 2>(a, tk, tv, like, st);
+  // As many column tiles as hold a decode group (16 columns at a time beyond that), or a list's items
+  // on average, so that one pass over the keys does.  Lists of 64 items over 4000 keys, us with 1 / 2 /
+  // 3 column tiles: 8 rows 94 / 105 / 139, 12 rows 178 / 107 / 140, 20 rows 266 / 192 / 143, 32 rows
+  // 351 / 196 / 257 (two passes of 16 beat 24 + 8).
+  if (list && (rows > 24 || (rows > 8 && rows <= 16))) launch<true, 2>(a, tk, tv, like, st);
+  else if (list && rows > 16) launch<true, 3>(a, tk, tv, like, st);
+  else if (list) launch<true, 1>(a, tk, tv, like, st);
   else if (a.group <= 8) launch<false, 1>(a, tk, tv, like, st);
   else launch<false, 2>(a, tk, tv, like, st);
 }

@@ -95,12 +95,13 @@ std::vector<at::Tensor> step_tables(const at::Tensor& ctx_lens, const at::Tensor
                                     const at::Tensor& new_blocks, int64_t num_tokens,
                                     int64_t block_size, int64_t group, int64_t rows_per_tile,
                                     int64_t num_decode, at::Tensor& err);
-void rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& slots,
-                 const at::Tensor& cos_sin, at::Tensor& k_cache, at::Tensor& v_cache,
-                 at::Tensor& k_scale, at::Tensor& v_scale, at::Tensor& q_out, int64_t hq,
-                 int64_t hkv, const c10::optional<at::Tensor>& q_norm,
-                 const c10::optional<at::Tensor>& k_norm, int64_t norm_dim, double eps,
-                 at::Tensor& err);
+at::Tensor rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& slots,
+                       const at::Tensor& cos_sin, at::Tensor& k_cache, at::Tensor& v_cache,
+                       at::Tensor& k_scale, at::Tensor& v_scale,
+                       const c10::optional<at::Tensor>& out, int64_t hq, int64_t hkv,
+                       const c10::optional<at::Tensor>& q_norm,
+                       const c10::optional<at::Tensor>& k_norm, int64_t norm_dim, double eps,
+                       at::Tensor& err);
 void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
                          const at::Tensor& v_cache, const at::Tensor& k_scale,
                          const at::Tensor& v_scale, at::Tensor& out,

@@ -11,6 +11,7 @@
 // tokens alone (what it held belongs to a former owner).
 //
 // k and v are rounded once, from fp32 after norm and rotation.
+#include <ATen/Functions.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -440,12 +441,13 @@ void check_fp8_cache(const char* op, const at::Tensor& k_cache, const at::Tensor
               ": KV pool rows exceed int32");
 }
 
-void rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& slots,
-                 const at::Tensor& cos_sin, at::Tensor& k_cache, at::Tensor& v_cache,
-                 at::Tensor& k_scale, at::Tensor& v_scale, at::Tensor& q_out, int64_t hq,
-                 int64_t hkv, const c10::optional<at::Tensor>& q_norm,
-                 const c10::optional<at::Tensor>& k_norm, int64_t norm_dim, double eps,
-                 at::Tensor& err) {
+at::Tensor rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& slots,
+                       const at::Tensor& cos_sin, at::Tensor& k_cache, at::Tensor& v_cache,
+                       at::Tensor& k_scale, at::Tensor& v_scale,
+                       const c10::optional<at::Tensor>& out, int64_t hq, int64_t hkv,
+                       const c10::optional<at::Tensor>& q_norm,
+                       const c10::optional<at::Tensor>& k_norm, int64_t norm_dim, double eps,
+                       at::Tensor& err) {
   using namespace kq;
   check_fp8_cache("rope_kv_fp8", k_cache, v_cache, k_scale, v_scale);
   const int64_t T = qkv.size(0), R = cos_sin.size(1);
@@ -454,6 +456,8 @@ void rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const at::T
                   qkv.size(1) >= (hq + 2 * hkv) * D && (T <= 1 || qkv.stride(0) % 8 == 0) &&
                   qkv.stride(1) == 1 && reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
               "rope_kv_fp8: qkv bf16 [T, (hq + 2 hkv) 128], 16-byte aligned rows");
+  at::Tensor q_out =
+      out.has_value() && out->defined() ? *out : at::empty({T, hq, D}, qkv.options());
   TORCH_CHECK(q_out.is_cuda() && q_out.scalar_type() == at::kBFloat16 && q_out.dim() == 3 &&
                   q_out.size(0) == T && q_out.size(1) == hq && q_out.size(2) == D &&
                   q_out.stride(2) == 1 && q_out.stride(1) == D &&
@@ -479,7 +483,7 @@ void rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const at::T
     (i == 0 ? a.q_norm : a.k_norm) =
         has ? reinterpret_cast<const bf16*>(w->data_ptr()) : nullptr;
   }
-  if (T == 0) return;
+  if (T == 0) return q_out;
   a.qkv = reinterpret_cast<const bf16*>(qkv.data_ptr());
   a.ld = qkv.stride(0);
   a.positions = positions.data_ptr<int>();
@@ -517,6 +521,7 @@ void rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const at::T
   C10_CUDA_CHECK(launch_k(kernel, dim3(kv + qw), dim3(THREADS), 0,
                           at::cuda::getCurrentCUDAStream(), nullptr, 0, a, win,
                           static_cast<int>(kv)));
+  return q_out;
 }
 
 }  // namespace lb

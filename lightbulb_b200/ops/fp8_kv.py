@@ -24,6 +24,18 @@ FP8_MAX = 448.0                            # largest e4m3 value
 FP8_SCALE_MIN_EXP, FP8_SCALE_MAX_EXP = -40, 119
 
 
+_err_words: dict = {}       # device index -> error word of its scratch
+
+
+def _err(t: torch.Tensor) -> torch.Tensor:
+    """The error word of ``t``'s device (the scratch's; looked up once per device)."""
+    i = t.get_device()
+    w = _err_words.get(i)
+    if w is None:
+        w = _err_words[i] = scratch(t.device).err
+    return w
+
+
 class StepTables(NamedTuple):
     """Device-side integers of one step (all int32); see :func:`step_tables`."""
 
@@ -62,7 +74,7 @@ def step_tables(ctx_lens: torch.Tensor, q_lens: torch.Tensor, rows: Optional[tor
     if ctx_lens.is_cuda:
         out = StepTables(*_need_c().step_tables(
             ctx_lens, q_lens, rows, seq_tables, new_blocks, num_tokens, block_size, group,
-            rows_per_tile, num_decode, scratch(ctx_lens.device).err))
+            rows_per_tile, num_decode, _err(ctx_lens)))
         _launches[0] += 1
         return out
     tiles = num_tokens * group // rows_per_tile + b
@@ -120,15 +132,15 @@ def rope_kv_fp8(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
     does not count as stored, and the rows that go to one block lie within ``block_size``
     consecutive rows, offsets rising.  Infinities are stored as the largest magnitude, NaN as
     NaN."""
+    if qkv.is_cuda:
+        _launches[0] += 1
+        return _need_c().rope_kv_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale,
+                                     v_scale, out, hq, hkv, q_norm, k_norm, norm_dim, eps,
+                                     _err(qkv))
+    # CPU restatement
     t, d = qkv.shape[0], k_cache.shape[-1]
     if out is None:
-        out = torch.empty(t, hq, d, dtype=qkv.dtype, device=qkv.device)
-    if qkv.is_cuda:
-        _need_c().rope_kv_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale, v_scale,
-                              out, hq, hkv, q_norm, k_norm, norm_dim, eps, scratch(qkv.device).err)
-        _launches[0] += 1
-        return out
-    # CPU restatement
+        out = torch.empty(t, hq, d, dtype=qkv.dtype)
     r, bs = cos_sin.shape[1], k_cache.shape[2]
     half = r // 2
     x = qkv[:, :(hq + 2 * hkv) * d].reshape(t, hq + 2 * hkv, d).float()
@@ -185,7 +197,7 @@ def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     if q.is_cuda:
         _need_c().paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, out, block_tables,
                                       seq_lens, cu_q, tile_seq, tile_row0, group, scale, decode,
-                                      causal, scratch(q.device).err)
+                                      causal, _err(q))
         _launches[0] += 1
         return out
     # CPU restatement
