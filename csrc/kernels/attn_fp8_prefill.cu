@@ -550,30 +550,42 @@ __global__ void __launch_bounds__(THREADS, 1)
         m_used = m_new;
       }
       const float ms = SHIFT - (m_used == -INFINITY ? 0.f : m_used);
+      // exponents first, in place: the exponentials then follow each other without waiting
+#pragma unroll
+      for (int i = 0; i < NSL; ++i) {
+        const float add = lv[i] + ms;
+        const uint64_t sc2 = pack_f2(sc[i], sc[i]), ad2 = pack_f2(add, add);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const int e = 16 * i + 2 * c;
+          float x0, x1;
+          unpack_f2(fma_f2(pack_f2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), sc2, ad2),
+                    x0, x1);
+          sr[e] = __float_as_uint(x0);
+          sr[e + 1] = __float_as_uint(x1);
+        }
+      }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         uint32_t pk[16];
 #pragma unroll
-        for (int i2 = 0; i2 < 2; ++i2) {
-          const int i = 2 * q + i2;
-          const float add = lv[i] + ms;
-          const uint64_t sc2 = pack_f2(sc[i], sc[i]), ad2 = pack_f2(add, add);
-          uint64_t l2 = pack_f2(0.f, 0.f);
+        for (int c = 0; c < 32; ++c) sr[32 * q + c] = __float_as_uint(ex2(__uint_as_float(sr[32 * q + c])));
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const int e = 16 * i + 2 * c;
-            float x0, x1;
-            unpack_f2(fma_f2(pack_f2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), sc2, ad2),
-                      x0, x1);
-            const float p0 = ex2(x0), p1 = ex2(x1);
-            l2 = add_f2(l2, pack_f2(p0, p1));
-            pk[8 * i2 + c] = pack_f16x2(p0, p1);
-          }
-          float la, lb;
-          unpack_f2(l2, la, lb);
-          l = fmaf(la + lb, cst[i].z, l);
-        }
+        for (int c = 0; c < 16; ++c)
+          pk[c] = pack_f16x2(__uint_as_float(sr[32 * q + 2 * c]), __uint_as_float(sr[32 * q + 2 * c + 1]));
         tmem_st16(tl + colP + 16 * q, pk);
+#pragma unroll
+        for (int i2 = 0; i2 < 2; ++i2) {
+          const uint32_t* p = sr + 32 * q + 16 * i2;
+          uint64_t t4[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            t4[c] = add_f2(pack_f2(__uint_as_float(p[4 * c]), __uint_as_float(p[4 * c + 1])),
+                           pack_f2(__uint_as_float(p[4 * c + 2]), __uint_as_float(p[4 * c + 3])));
+          float la, lb;
+          unpack_f2(add_f2(add_f2(t4[0], t4[1]), add_f2(t4[2], t4[3])), la, lb);
+          l = fmaf(la + lb, cst[2 * q + i2].z, l);
+        }
       }
       tc_wait_st();
       tc_fence_before();
