@@ -27,6 +27,12 @@
 // 12 (then 13, 14, 15, 8 .. 11): both ldmatrix shapes then touch eight different swizzle rows.
 // Weights are f16 (11 bits) scaled to 2^15 at most, which keeps those bits down to 2^-29 of the
 // largest; vs enters through them relative to the largest vs so far.  m, l, O are fp32.
+//
+// Measured (32 query / 8 KV heads unless said): 256 ragged sequences up to 2304 keys 117 us (5.4 TB/s,
+// 84 % of the measured copy rate; the main kernel alone 106 us), 37 x 3001 with 32 KV heads 84 us (87 %),
+// 7 sequences up to 100k keys with 64 / 8 heads 131 us (88 %), one of 2047 keys 11.8 us (launches and
+// the first loads), 32 x up to 5 tokens over up to 1280 keys 29 us.  With 8 warps an SM instead of 12
+// the first took 126 us: two warps a scheduler leave it idle most of the time.
 #include <ATen/Functions.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>

@@ -11,6 +11,11 @@
 // tokens alone (what it held belongs to a former owner).
 //
 // k and v are rounded once, from fp32 after norm and rotation.
+//
+// HBM traffic is qkv in, q and codes out (167 MB for 7.1k rows of 32 + 8 + 8 heads: 25.9 us at the
+// measured copy rate); instructions bind it first.  Measured: 7.1k rows with norms 45.5 us (3.7 TB/s,
+// 57 %), 256 decode rows 4.1 us, one row 3.0 us.  Tried: a warp holding 16 rows of a block 92 us
+// (spills), lanes exchanging rotation partners by shuffle 65 us, 8 q heads per warp 49 us.
 #include <ATen/Functions.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>

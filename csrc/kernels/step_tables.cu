@@ -15,7 +15,9 @@
 // shuffle scan per 256 requests; the lengths come from L2) and then fills its own share of
 // tokens, table entries and tiles, finding the owner of an item by bisection in shared memory.
 // A slot in a block that this step adds is taken from new_blocks, never from the table that
-// another CTA is writing.
+// another CTA is writing.  Table rows are copied in pieces of 128 entries per warp: with a warp per
+// row, 40 rows of 1907 entries took 13.9 us.  Measured: 3.6 us for 256 requests of one token, 3.4 us
+// for 40 chunks of up to 512 tokens behind 30,000; a launch that does nothing takes about 2.
 #include <ATen/Functions.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
