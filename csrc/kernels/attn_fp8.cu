@@ -8,6 +8,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
 
 #include "attn_fp8.cuh"
 
@@ -27,6 +28,7 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   using namespace fp8a;
   const char* op = "paged_attention_fp8";
   check_fp8_cache(op, k_cache, v_cache, k_scale, v_scale);
+  const c10::cuda::CUDAGuard guard(k_cache.device());
   for (const at::Tensor* t : {&q, (const at::Tensor*)&out})
     TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kBFloat16 && t->dim() == 3 &&
                     t->size(2) == D && t->stride(2) == 1 && (t->size(1) <= 1 || t->stride(1) == D) &&
@@ -61,6 +63,7 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   a.log2_bs = k_cache.size(2) == 16 ? 4 : k_cache.size(2) == 32 ? 5 : 6;
   a.num_blocks = k_cache.size(0);
   a.num_seqs = B;
+  a.tokens = static_cast<int>(q.size(0));
   a.causal = causal ? 1 : 0;
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   a.err = err.data_ptr<int>();

@@ -33,6 +33,7 @@ struct Args {
   const int* tile_row0;
   int num_tiles;
   int hq, hkv, group, log2_bs, num_blocks, num_seqs;
+  int tokens;             // rows of q and out
   int causal;
   float scale_log2;
   int* err;
@@ -67,6 +68,15 @@ __device__ __forceinline__ int q_shift(float amax) {
   return amax > 0.f ? min(126, max(-112, 14 - e)) : 0;
 }
 __device__ __forceinline__ float pow2i(int k) { return __uint_as_float((k + 127) << 23); }
+
+// cudaFuncSetAttribute holds for one device: true the first time on the current one.
+inline bool first_on_device(bool (&done)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 64 && done[dev]) return false;
+  if (dev < 64) done[dev] = true;
+  return true;
+}
 
 // Physical block of slice `s` (16 keys) of a sequence; an id outside the pool is reported and
 // replaced by block 0, so every TMA coordinate stays inside the tensor map.

@@ -237,7 +237,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   const bool used = seq >= 0 && !bad;
   if (bad && threadIdx.x == 0) record_error(a.err, kErrBounds);
   const int q_start = used ? a.cu_q[seq] : 0;
-  const int q_len = used ? a.cu_q[seq + 1] - q_start : 0;
+  int q_len = used ? a.cu_q[seq + 1] - q_start : 0;
+  if (q_start < 0 || q_len < 0 || q_len > a.tokens - q_start) {
+    if (threadIdx.x == 0) record_error(a.err, kErrBounds);
+    q_len = 0;
+  }
   int kv_len = used ? max(0, a.seq_lens[seq]) : 0;
   const int64_t cap = static_cast<int64_t>(a.bt_width) << a.log2_bs;
   if (kv_len > cap) {
@@ -666,12 +670,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 void fp8_prefill(const fp8a::Args& a, const CUtensorMap& tk, const CUtensorMap& tv,
                  cudaStream_t st) {
   using namespace fp8p;
-  static bool attr = false;
-  if (!attr) {
+  static bool attr[64] = {};
+  if (first_on_device(attr))
     C10_CUDA_CHECK(cudaFuncSetAttribute(prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         SMEM_TOTAL));
-    attr = true;
-  }
   C10_CUDA_CHECK(launch_k(prefill_kernel, dim3(a.num_tiles, a.hkv), dim3(THREADS), SMEM_TOTAL, st,
                           nullptr, 0, tk, tv, a));
 }

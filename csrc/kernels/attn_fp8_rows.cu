@@ -158,7 +158,11 @@ __device__ void scan_entries(const Args& a, const Entries<LIST>& en, int* s_tot)
         int q0 = 0, rows = 0, lo = 0;
         if (seq >= 0) {
           q0 = a.cu_q[seq];
-          const int n = a.cu_q[seq + 1] - q0;
+          int n = a.cu_q[seq + 1] - q0;
+          if (q0 < 0 || n < 0 || n > a.tokens - q0) {
+            record_error(a.err, kErrBounds);
+            n = 0;
+          }
           rows = max(0, min(n * a.group - row0, ENTRY_ROWS));
           lim = max(0, a.seq_lens[seq]);
           if (lim > cap) {
@@ -734,12 +738,10 @@ void launch(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const a
   wk.entries = LIST ? a.num_tiles : a.num_seqs;
   const size_t lens = WARPS * sizeof(int) + Entries<LIST>::bytes(wk.entries);
   const size_t smem = 1024 + WARPS * (WARP_SMEM + q_smem_of(NT)) + WARPS * STAGES * 24 + lens;
-  static bool attr = false;
-  if (!attr) {
+  static bool attr[64] = {};
+  if (first_on_device(attr))
     C10_CUDA_CHECK(cudaFuncSetAttribute(rows_kernel<LIST, NT>,
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    attr = true;
-  }
   // fewer CTAs an SM when the entries' tables of a very large batch need the room; no more warps
   // than the tiles there can be make shares
   const int per_sm = std::max<int>(1, std::min<size_t>(ctas_of(NT), 228 * 1024 / (smem + 1024)));

@@ -20,6 +20,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
 
 #include "common.cuh"
 
@@ -455,6 +456,7 @@ at::Tensor rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const
                        at::Tensor& err) {
   using namespace kq;
   check_fp8_cache("rope_kv_fp8", k_cache, v_cache, k_scale, v_scale);
+  const c10::cuda::CUDAGuard guard(k_cache.device());
   const int64_t T = qkv.size(0), R = cos_sin.size(1);
   TORCH_CHECK(hq >= 1 && hkv >= 1 && k_cache.size(1) == hkv, "rope_kv_fp8: head counts");
   TORCH_CHECK(qkv.is_cuda() && qkv.dim() == 2 && qkv.scalar_type() == at::kBFloat16 &&

@@ -22,6 +22,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
 
 #include "common.cuh"
 
@@ -224,6 +225,7 @@ std::vector<at::Tensor> step_tables(const at::Tensor& ctx_lens, const at::Tensor
   TORCH_CHECK(seq_tables.is_cuda() && seq_tables.scalar_type() == at::kInt &&
                   seq_tables.dim() == 2 && (seq_tables.size(1) <= 1 || seq_tables.stride(1) == 1),
               "step_tables: seq_tables [S, W] int32, contiguous rows");
+  const c10::cuda::CUDAGuard guard(ctx_lens.device());
   const int64_t W = seq_tables.size(1);
   const bool has_rows = rows.has_value() && rows->defined();
   if (has_rows)

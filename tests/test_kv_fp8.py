@@ -600,6 +600,23 @@ def test_attention_reports_bad_blocks(decode):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cu", [[0, 300], [-1, 3], [2, 1]])
+@pytest.mark.parametrize("pad_tiles", [0, 20])        # both kernels: 9 or 189 rows per item
+def test_prefill_reports_offsets_outside_q(cu, pad_tiles):
+    kc, vc, ks, vs, tables = _paged_inputs([100], 1, 16, 1)
+    q = torch.randn(3, 63, D, device="cuda").bfloat16()
+    out = torch.full_like(q, 3.0)
+    tiles = [0] + [-1] * pad_tiles
+    ops.paged_attention_fp8(q, *(z.cuda() for z in (kc, vc, ks, vs)), _i32(tables, "cuda"),
+                            _i32([100], "cuda"), _i32(cu, "cuda"), out, 63, False,
+                            tile_seq=_i32(tiles, "cuda"), tile_row0=_i32([0] * len(tiles), "cuda"))
+    torch.cuda.synchronize()
+    with pytest.raises(ops.KernelError):
+        ops.check_errors()
+    assert bool((out == 3).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("decode", [True, False])
 def test_attention_other_stream_and_graph(decode):
     kc, vc, ks, vs, tables = _paged_inputs([3000, 40], 2, 16, 1)
