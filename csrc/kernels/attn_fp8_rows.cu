@@ -28,10 +28,10 @@
 // Weights are f16 (11 bits) scaled to 2^15 at most, which keeps those bits down to 2^-29 of the
 // largest; vs enters through them relative to the largest vs so far.  m, l, O are fp32.
 //
-// Measured (32 query / 8 KV heads unless said): 256 ragged sequences up to 2304 keys 117 us (5.4 TB/s,
-// 84 % of the measured copy rate; the main kernel alone 106 us), 37 x 3001 with 32 KV heads 84 us (87 %),
-// 7 sequences up to 100k keys with 64 / 8 heads 131 us (88 %), one of 2047 keys 11.8 us (launches and
-// the first loads), 32 x up to 5 tokens over up to 1280 keys 29 us.  With 8 warps an SM instead of 12
+// Measured (32 query / 8 KV heads unless said): 256 ragged sequences up to 2304 keys 115 us (5.6 TB/s,
+// 86 % of the measured copy rate; the main kernel alone 106 us), 37 x 3001 with 32 KV heads 83 us (89 %),
+// 7 sequences up to 100k keys with 64 / 8 heads 130 us (88 %), one of 2047 keys 10.3 us (launches and
+// the first loads), 32 x up to 5 tokens over up to 1280 keys 30 us.  With 8 warps an SM instead of 12
 // the first took 126 us: two warps a scheduler leave it idle most of the time.
 #include <ATen/Functions.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -58,7 +58,6 @@ constexpr int ctas_of(int nt) { return nt == 1 ? 3 : 2; }
 constexpr int q_smem_of(int nt) { return nt > 2 ? nt * 8 * 32 * 8 : 0; }    // bytes per warp
 constexpr int MAX_ENTRIES = 4096;
 constexpr int ENTRY_ROWS = 256;               // packed query rows of a work list's item
-constexpr int MIN_TILES = 4;                  // per share: less is not worth a partial result
 constexpr float P_TOP = 32768.f;              // weights are p * 2^15
 
 // A run that starts in a share and goes on in the next ones, for the kernel that joins its parts.
@@ -137,12 +136,13 @@ struct Entries {
   static size_t bytes(int n) { return (static_cast<size_t>(FIELDS) * n + 1) * sizeof(int); }
 };
 
-// Fills the entries; every thread of the CTA takes part.  HT: columns per chunk.
+// Fills the entries; every thread of the CTA takes part.  HT: columns per chunk.  Returns the number
+// of runs.
 template <bool LIST, int HT>
-__device__ void scan_entries(const Args& a, const Entries<LIST>& en, int* s_tot) {
+__device__ int scan_entries(const Args& a, const Entries<LIST>& en, int* s_tot) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t cap = static_cast<int64_t>(a.bt_width) << a.log2_bs;
-  int base = 0;
+  int base = 0, total_runs = 0;
   for (int e0 = 0; e0 < en.n; e0 += THREADS) {
     const int e = e0 + tid;
     int lim = 0, runs = a.hkv * ((a.group + HT - 1) / HT);
@@ -195,23 +195,34 @@ __device__ void scan_entries(const Args& a, const Entries<LIST>& en, int* s_tot)
       const int up = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += up;
     }
-    if (lane == 31) s_tot[warp] = v;
+    const int r = __reduce_add_sync(0xffffffffu, lim > 0 ? runs : 0);
+    if (lane == 31) {
+      s_tot[warp] = v;
+      s_tot[WARPS + warp] = r;
+    }
     __syncthreads();
     int all = 0;
     for (int w = 0; w < WARPS; ++w) {
       if (w < warp) v += s_tot[w];
       all += s_tot[w];
+      total_runs += s_tot[WARPS + w];
     }
     if (e < en.n) en.cum[e + 1] = base + v;
     if (e == 0) en.cum[0] = 0;
     base += all;
     __syncthreads();
   }
+  return total_runs;
 }
 
-// Shares: worker w of n takes units [w U / n, (w + 1) U / n).
-__device__ __forceinline__ int active_workers(int units, int workers) {
-  return max(1, min(workers, units / MIN_TILES));
+// Shares: worker w of n takes units [w U / n, (w + 1) U / n).  While there are fewer tiles than the
+// warps could take, a longer share costs its warp about a microsecond a tile and a shorter one gives
+// the join more parts: sqrt(tiles of a run) / 4 tiles a share balances them.  us with 1 / 2 / 4 / 8 (8
+// KV heads): 1 x 300 keys 7.7 / 8.4 / 11.6 / 16.5, 1 x 2047 11.7 / 10.4 / 11.9 / 16.2, 1 x 8000 27.4 /
+// 19.4 / 16.8 / 18.9, 1 x 30000 35 / 35 / 35 / 29.
+__device__ __forceinline__ int active_workers(int units, int runs, int workers) {
+  const int tiles = max(1, __float2int_rn(0.25f * sqrtf(__fdividef(units, max(1, runs)))));
+  return max(1, min(workers, units / tiles));
 }
 __device__ __forceinline__ int share_begin(int w, int units, int n) {
   return static_cast<int>(static_cast<int64_t>(w) * units / n);
@@ -289,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
   float* s_scale = reinterpret_cast<float*>(smem + META + WARPS * STAGES * 8) +
                    warp * STAGES * 4;
   int* s_tot = reinterpret_cast<int*>(smem + META + WARPS * STAGES * 24);
-  const Entries<LIST> en(s_tot + WARPS, wk.entries);
+  const Entries<LIST> en(s_tot + 2 * WARPS, wk.entries);
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 3);   // lane 0's expect + two scale loads
     fence_barrier_init();
@@ -300,7 +311,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
   pdl_trigger();
   const int w = warp * gridDim.x + blockIdx.x;   // neighbours on the line sit on different SMs
   if (lane == 0) wk.cut[w].parts = 0;
-  scan_entries<LIST, HT>(a, en, s_tot);
+  const int all_runs = scan_entries<LIST, HT>(a, en, s_tot);
   // rows that see no key give 0
   for (int e = blockIdx.x; e < en.n; e += gridDim.x) {
     if (en.lim[e] > 0) continue;                                    // CTA-uniform
@@ -315,7 +326,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
   const int units = en.cum[en.n];
   if (units == 0) return;
   const int runs = a.hkv * ((a.group + HT - 1) / HT);   // of a decode entry
-  const int n_act = active_workers(units, wk.workers);
+  const int n_act = active_workers(units, all_runs, wk.workers);
   if (w >= n_act) return;
   const int u_begin = share_begin(w, units, n_act), u_end = share_begin(w + 1, units, n_act);
   if (u_begin >= u_end) return;
@@ -736,7 +747,7 @@ void launch(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const a
   constexpr int HT = 8 * NT, STAGES = stages_of(NT), WARP_SMEM = STAGES * STAGE;
   Work wk;
   wk.entries = LIST ? a.num_tiles : a.num_seqs;
-  const size_t lens = WARPS * sizeof(int) + Entries<LIST>::bytes(wk.entries);
+  const size_t lens = 2 * WARPS * sizeof(int) + Entries<LIST>::bytes(wk.entries);
   const size_t smem = 1024 + WARPS * (WARP_SMEM + q_smem_of(NT)) + WARPS * STAGES * 24 + lens;
   static bool attr[64] = {};
   if (first_on_device(attr))
@@ -747,7 +758,7 @@ void launch(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const a
   const int per_sm = std::max<int>(1, std::min<size_t>(ctas_of(NT), 228 * 1024 / (smem + 1024)));
   const int64_t tiles = line_bound(a, LIST, HT);
   const int grid = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>(148 * per_sm, (tiles + MIN_TILES - 1) / MIN_TILES)));
+      std::max<int64_t>(1, std::min<int64_t>(148 * per_sm, (tiles + WARPS - 1) / WARPS)));
   wk.workers = grid * WARPS;
   static_assert(sizeof(Cut) % 8 == 0, "the partials follow the cuts");
   const int64_t part_rows = static_cast<int64_t>(wk.workers) * 2 * HT;
