@@ -648,6 +648,40 @@ def test_attention_other_stream_and_graph(decode):
     ops.check_errors()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,n_q,bs", [([320], [200], 16), ([513, 40], [200, 40], 32),
+                                         ([1025, 1, 640], [1, 1, 1], 64), ([900] * 30, [3] * 30, 16)])
+def test_attention_same_bits_cold_and_warm(lens, n_q, bs):
+    """The pipelines' timing changes with what is in L2; the results do not."""
+    hq, hkv = 8, 2
+    kc, vc, ks, vs, tables = _paged_inputs(lens, hkv, bs, 7)
+    args = [z.cuda() for z in (kc, vc, ks, vs)]
+    t, decode = sum(n_q), max(n_q) == 1
+    q = torch.randn(t, hq, D, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    cu = [0]
+    for m in n_q:
+        cu.append(cu[-1] + m)
+    tiles = [(i, r) for i, m in enumerate(n_q) for r in range(0, m * 4, 256)]
+    idx = [_i32(v, "cuda") for v in (tables, lens, cu)]
+    ts, tr = _i32([a for a, _ in tiles], "cuda"), _i32([r for _, r in tiles], "cuda")
+    flush = torch.empty(48 << 20, dtype=torch.int32, device="cuda")
+    first = None
+    for i in range(40):
+        if i % 2:
+            flush.fill_(i)
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        ops.paged_attention_fp8(q, *args, *idx, out, 4, decode, tile_seq=ts, tile_row0=tr)
+        torch.cuda.synchronize()
+        if first is None:
+            first = out.clone()
+            ref, tol = _attention_ref(q.cpu(), kc, vc, ks, vs, tables, lens, n_q, 4, not decode,
+                                      None)
+            assert bool(((out.cpu().double() - ref).abs() <= tol).all())
+        assert torch.equal(out, first), i
+    ops.check_errors()
+
+
 # --------------------------------------------------------------------------------------
 # refusals
 # --------------------------------------------------------------------------------------
