@@ -17,14 +17,15 @@ namespace lb {
 void check_fp8_cache(const char* op, const at::Tensor& k_cache, const at::Tensor& v_cache,
                      const at::Tensor& k_scale, const at::Tensor& v_scale);
 
-void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
-                         const at::Tensor& v_cache, const at::Tensor& k_scale,
-                         const at::Tensor& v_scale, at::Tensor& out,
-                         const at::Tensor& block_tables, const at::Tensor& seq_lens,
-                         const c10::optional<at::Tensor>& cu_q,
-                         const c10::optional<at::Tensor>& tile_seq,
-                         const c10::optional<at::Tensor>& tile_row0, int64_t group, double scale,
-                         bool decode, bool causal, at::Tensor& err) {
+// Returns the number of kernels launched.
+int64_t paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
+                            const at::Tensor& v_cache, const at::Tensor& k_scale,
+                            const at::Tensor& v_scale, at::Tensor& out,
+                            const at::Tensor& block_tables, const at::Tensor& seq_lens,
+                            const c10::optional<at::Tensor>& cu_q,
+                            const c10::optional<at::Tensor>& tile_seq,
+                            const c10::optional<at::Tensor>& tile_row0, int64_t group, double scale,
+                            bool decode, bool causal, at::Tensor& err) {
   using namespace fp8a;
   const char* op = "paged_attention_fp8";
   check_fp8_cache(op, k_cache, v_cache, k_scale, v_scale);
@@ -76,11 +77,11 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   if (decode) {
     TORCH_CHECK(q.size(0) >= B, op, ": one query token per sequence");
-    if (B == 0) return;
+    if (B == 0) return 0;
     TORCH_CHECK(fp8_rows_fits(a, false), op,
                 ": at most 4096 sequences, and 2^31 / 32 keys x KV heads in their tables");
     fp8_rows(a, false, group, tk, tv, q, st);
-    return;
+    return 2;
   }
   TORCH_CHECK(cu_q.has_value() && tile_seq.has_value() && tile_row0.has_value(), op,
               ": prefill needs cu_q and the work list (tile_seq, tile_row0)");
@@ -88,7 +89,7 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
     TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kInt && t->is_contiguous(), op,
                 ": cu_q and the work list are contiguous int32");
   TORCH_CHECK(cu_q->numel() >= B + 1 && tile_seq->numel() == tile_row0->numel(), op, ": sizes");
-  if (B == 0 || tile_seq->numel() == 0) return;
+  if (B == 0 || tile_seq->numel() == 0) return 0;
   a.cu_q = cu_q->data_ptr<int>();
   a.tile_seq = tile_seq->data_ptr<int>();
   a.tile_row0 = tile_row0->data_ptr<int>();
@@ -98,10 +99,12 @@ void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   // 32 x 1280 49 / 52; 48 rows 32 x 1280 64 / 52; 64 rows 81 / 52.
   constexpr int64_t FEW_ROWS = 32;
   const int64_t avg = (q.size(0) * group + a.num_tiles - 1) / a.num_tiles;
-  if (avg <= FEW_ROWS && fp8_rows_fits(a, true))
+  if (avg <= FEW_ROWS && fp8_rows_fits(a, true)) {
     fp8_rows(a, true, avg, tk, tv, q, st);
-  else
-    fp8_prefill(a, tk, tv, st);
+    return 2;
+  }
+  fp8_prefill(a, tk, tv, st);
+  return 1;
 }
 
 }  // namespace lb

@@ -8,7 +8,7 @@
 // in flight on every SM and to spend few instructions per byte.
 //
 // Work split.  An entry is a sequence (decode) or an item of the work list; its query rows (token,
-// head in group) are cut into chunks of 8 or 16 columns, and (KV head, chunk) over the entry's keys
+// head in group) are cut into chunks of 8, 16 or 24 columns, and (KV head, chunk) over the entry's keys
 // is a run of 32-key tiles.  All runs form one line; each warp takes an equal, contiguous share of
 // it (the sum over the lengths is repeated by every CTA, so no host length and no plan is needed).
 // Ragged batches, a single long sequence and many short ones all load the SMs evenly.  A run that

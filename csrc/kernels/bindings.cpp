@@ -102,14 +102,14 @@ at::Tensor rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const
                        const c10::optional<at::Tensor>& q_norm,
                        const c10::optional<at::Tensor>& k_norm, int64_t norm_dim, double eps,
                        at::Tensor& err);
-void paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
-                         const at::Tensor& v_cache, const at::Tensor& k_scale,
-                         const at::Tensor& v_scale, at::Tensor& out,
-                         const at::Tensor& block_tables, const at::Tensor& seq_lens,
-                         const c10::optional<at::Tensor>& cu_q,
-                         const c10::optional<at::Tensor>& tile_seq,
-                         const c10::optional<at::Tensor>& tile_row0, int64_t group, double scale,
-                         bool decode, bool causal, at::Tensor& err);
+int64_t paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
+                            const at::Tensor& v_cache, const at::Tensor& k_scale,
+                            const at::Tensor& v_scale, at::Tensor& out,
+                            const at::Tensor& block_tables, const at::Tensor& seq_lens,
+                            const c10::optional<at::Tensor>& cu_q,
+                            const c10::optional<at::Tensor>& tile_seq,
+                            const c10::optional<at::Tensor>& tile_row0, int64_t group, double scale,
+                            bool decode, bool causal, at::Tensor& err);
 }  // namespace lb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

@@ -195,10 +195,9 @@ def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     if scale is None:
         scale = 1.0 / math.sqrt(d)
     if q.is_cuda:
-        _need_c().paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, out, block_tables,
-                                      seq_lens, cu_q, tile_seq, tile_row0, group, scale, decode,
-                                      causal, _err(q))
-        _launches[0] += 1
+        _launches[0] += _need_c().paged_attention_fp8(
+            q, k_cache, v_cache, k_scale, v_scale, out, block_tables, seq_lens, cu_q, tile_seq,
+            tile_row0, group, scale, decode, causal, _err(q))
         return out
     # CPU restatement
     from ..models.reference import attention_ref
