@@ -60,6 +60,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // q enters the tensor cores as f16 (K's codes are exact there).  Each row is first scaled by a
 // power of two that brings its largest element to [2^14, 2^15): bf16's 8 bits then fit f16's 11
 // for every element down to 2^-32 of the largest.  Returns the exponent of that power.

@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_after();
     }
     if (ok && t < nqt) {
-      const float inv = l != 0.f ? vs0 / l : 0.f;
+      const float inv = l != 0.f ? 1.f / l : 0.f;
       bf16* dst = a.out + static_cast<int64_t>(q_start + tok) * a.out_ld +
                   static_cast<int64_t>(head) * D;
 #pragma unroll 1
@@ -635,12 +635,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (valid_row) {
 #pragma unroll
+          for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * inv * vs0);
+#pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint4 v;
-            v.x = pack_bf16x2(__uint_as_float(ov[8 * i]) * inv, __uint_as_float(ov[8 * i + 1]) * inv);
-            v.y = pack_bf16x2(__uint_as_float(ov[8 * i + 2]) * inv, __uint_as_float(ov[8 * i + 3]) * inv);
-            v.z = pack_bf16x2(__uint_as_float(ov[8 * i + 4]) * inv, __uint_as_float(ov[8 * i + 5]) * inv);
-            v.w = pack_bf16x2(__uint_as_float(ov[8 * i + 6]) * inv, __uint_as_float(ov[8 * i + 7]) * inv);
+            v.x = pack_bf16x2(__uint_as_float(ov[8 * i]), __uint_as_float(ov[8 * i + 1]));
+            v.y = pack_bf16x2(__uint_as_float(ov[8 * i + 2]), __uint_as_float(ov[8 * i + 3]));
+            v.z = pack_bf16x2(__uint_as_float(ov[8 * i + 4]), __uint_as_float(ov[8 * i + 5]));
+            v.w = pack_bf16x2(__uint_as_float(ov[8 * i + 6]), __uint_as_float(ov[8 * i + 7]));
             *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = v;
           }
         }

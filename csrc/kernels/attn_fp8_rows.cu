@@ -1,8 +1,8 @@
 // Attention over the 8-bit paged KV cache for few query rows per sequence (sm_100a): decode (one
 // token) and short chunks such as speculative verification.
 //
-//   s_j = scale * ks_{b(j)} (q . k8_j),   m = max_j s_j,   p_j = 2^(s_j - m),  l = sum_j p_j
-//   o   = sum_j p_j vs_{b(j)} v8_j / l
+//   t_j = log2(e) scale * ks_{b(j)} (q . k8_j) + log2 vs_{b(j)},   m = max_j t_j,   w_j = 2^(t_j - m)
+//   o   = sum_j w_j v8_j / sum_j w_j / vs_{b(j)}
 //
 // HBM-bound: every cache byte is used once per few query rows, so the work is to keep enough bytes
 // in flight on every SM and to spend few instructions per byte.
@@ -26,7 +26,9 @@
 // one cvt per pair, with q and the keys permuted to match.  K's second 8-key group starts at key
 // 12 (then 13, 14, 15, 8 .. 11): both ldmatrix shapes then touch eight different swizzle rows.
 // Weights are f16 (11 bits) scaled to 2^15 at most, which keeps those bits down to 2^-29 of the
-// largest; vs enters through them relative to the largest vs so far.  m, l, O are fp32.
+// largest.  vs is part of a weight's exponent, so a block counts by its softmax weight times its scale,
+// however far its scale lies from the others'.  l sums w / vs relative to the share's first vs, so vs may
+// spread over 2^100 in a sequence and head.  m, l, O are fp32.
 //
 // Measured (32 query / 8 KV heads unless said): 256 ragged sequences up to 2304 keys 115 us (5.6 TB/s,
 // 86 % of the measured copy rate; the main kernel alone 106 us), 37 x 3001 with 32 KV heads 83 us (89 %),
@@ -58,7 +60,8 @@ constexpr int ctas_of(int nt) { return nt == 1 ? 3 : 2; }
 constexpr int q_smem_of(int nt) { return nt > 2 ? nt * 8 * 32 * 8 : 0; }    // bytes per warp
 constexpr int MAX_ENTRIES = 4096;
 constexpr int ENTRY_ROWS = 256;               // packed query rows of a work list's item
-constexpr float P_TOP = 32768.f;              // weights are p * 2^15
+constexpr float P_EXP = 15.f;                 // weights are w * 2^15
+constexpr float VS_SPREAD = 100.f;            // log2 of the largest ratio of V scales that l holds
 
 // A run that starts in a share and goes on in the next ones, for the kernel that joins its parts.
 struct Cut {
@@ -70,7 +73,7 @@ struct Cut {
 struct Work {
   Cut* cut;           // [workers]
   float* part_o;      // [2 workers][columns of a chunk][D]
-  float2* part_ml;    // [2 workers][columns of a chunk]
+  float4* part_ml;    // [2 workers][columns of a chunk]: m, l, log2 of the vs that l is relative to
   int workers;        // warps of the grid
   int entries;
 };
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
       hs[n][0] = __shfl_sync(0xffffffffu, down, t4 * 8);
       hs[n][1] = __shfl_sync(0xffffffffu, down, t4 * 8 + 4);
     }
-    float m[NT][2], l[NT][2], o[NT][8][4], vref = 7.5e-37f;   // 2^-120: below any useful scale
+    float m[NT][2], l[NT][2], o[NT][8][4], lv_ref = 0.f;   // lv_ref: log2 of the first tile's vs
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
@@ -459,7 +462,6 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.f;
     }
-    float inv_vref = P_TOP / vref;
 #pragma unroll 1
     for (int t = t0; t < t1; ++t) {
       ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, nullptr));
@@ -468,6 +470,9 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
       const int nsl = left > SL ? 2 : 1;
       const float2 sc0 = *reinterpret_cast<const float2*>(s_scale + stage * 4);
       const float2 sc1 = nsl > 1 ? *reinterpret_cast<const float2*>(s_scale + stage * 4 + 2) : sc0;
+      const float lv0 = lg2(sc0.y), lv1 = lg2(sc1.y);
+      if (t == t0) lv_ref = lv0;
+      const float rv0 = ex2(fminf(lv_ref - lv0, VS_SPREAD)), rv1 = ex2(fminf(lv_ref - lv1, VS_SPREAD));
       // ---- S^T = K Q^T ----
       float s[2][NT][4];
 #pragma unroll
@@ -503,13 +508,14 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
             mma_f16(s[i][n], y[0], y[1], y[2], y[3], h.x, h.y);
           }
         }
-        const float ks = i ? sc1.x : sc0.x;
+        const float ks = i ? sc1.x : sc0.x, lv = i ? lv1 : lv0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          s[i][n][0] *= ks * hs[n][0];
-          s[i][n][1] *= ks * hs[n][1];
-          s[i][n][2] *= ks * hs[n][0];
-          s[i][n][3] *= ks * hs[n][1];
+          const float f0 = ks * hs[n][0], f1 = ks * hs[n][1];
+          s[i][n][0] = fmaf(s[i][n][0], f0, lv);
+          s[i][n][1] = fmaf(s[i][n][1], f1, lv);
+          s[i][n][2] = fmaf(s[i][n][2], f0, lv);
+          s[i][n][3] = fmaf(s[i][n][3], f1, lv);
         }
       }
       if (see_min - t * KT < KT) {
@@ -539,25 +545,19 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
           corr[n][j] = ex2(m[n][j] - safe);
           moved |= mx != m[n][j];
           m[n][j] = mx;
+          const float top = safe - P_EXP;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            s[i][n][j] = ex2(s[i][n][j] - safe);
-            s[i][n][j + 2] = ex2(s[i][n][j + 2] - safe);
+            s[i][n][j] = ex2(s[i][n][j] - top);
+            s[i][n][j + 2] = ex2(s[i][n][j + 2] - top);
           }
-          l[n][j] = l[n][j] * corr[n][j] +
-                    ((s[0][n][j] + s[0][n][j + 2]) + (s[1][n][j] + s[1][n][j + 2]));
+          l[n][j] = fmaf(s[0][n][j] + s[0][n][j + 2], rv0,
+                         fmaf(s[1][n][j] + s[1][n][j + 2], rv1, l[n][j] * corr[n][j]));
         }
-      const float vmax = fmaxf(sc0.y, sc1.y);
-      float vcorr = 1.f;
-      if (vmax > vref) {                                  // warp-uniform
-        vcorr = vref / vmax;
-        vref = vmax;
-        inv_vref = P_TOP / vref;
-      }
-      if (__any_sync(0xffffffffu, moved || vcorr != 1.f)) {
+      if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const float c0 = corr[n][0] * vcorr, c1 = corr[n][1] * vcorr;
+          const float c0 = corr[n][0], c1 = corr[n][1];
 #pragma unroll
           for (int d = 0; d < 8; ++d) {
             o[n][d][0] *= c0;
@@ -571,12 +571,11 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (i < nsl) {
-          const float c = (i ? sc1.y : sc0.y) * inv_vref;
           uint32_t p[NT][2];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            p[n][0] = transpose8(pack_f16x2(s[i][n][0] * c, s[i][n][1] * c));
-            p[n][1] = transpose8(pack_f16x2(s[i][n][2] * c, s[i][n][3] * c));
+            p[n][0] = transpose8(pack_f16x2(s[i][n][0], s[i][n][1]));
+            p[n][1] = transpose8(pack_f16x2(s[i][n][2], s[i][n][3]));
           }
           const uint32_t base = v_addr + stage * STAGE + i * SLICE;
           auto add_v = [&](auto masked, uint32_t keep) {
@@ -622,13 +621,13 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
     const int slot = 2 * w + (t0 == 0 ? 1 : 0);
     if (t0 == 0 && !whole && lane == 0)
       wk.cut[w] = Cut{share_of(u + cc.nt - 1, units, n_act) - w + 1, co.count, co.row, co.kvh, co.q0};
-    const float vmul = vref * (1.f / P_TOP);
+    const float v_ref = ex2(lv_ref);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const float l0 = sum_over_keys(l[n][0]), l1 = sum_over_keys(l[n][1]);
       const int h0 = n * 8 + 2 * t4;
       if (whole) {
-        const float i0 = l0 != 0.f ? vmul / l0 : 0.f, i1 = l1 != 0.f ? vmul / l1 : 0.f;
+        const float i0 = l0 != 0.f ? 1.f / l0 : 0.f, i1 = l1 != 0.f ? 1.f / l1 : 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           if (h0 + j >= co.count) continue;
@@ -637,22 +636,22 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
           const float inv = j ? i1 : i0;
 #pragma unroll
           for (int d = 0; d < 8; ++d) {
-            dst[d * 16] = __float2bfloat16(o[n][d][j] * inv);
-            dst[d * 16 + 8] = __float2bfloat16(o[n][d][j + 2] * inv);
+            dst[d * 16] = __float2bfloat16(o[n][d][j] * inv * v_ref);
+            dst[d * 16 + 8] = __float2bfloat16(o[n][d][j + 2] * inv * v_ref);
           }
         }
       } else {
         float* dst = wk.part_o + (static_cast<int64_t>(slot) * HT + h0) * D + g;
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-          dst[d * 16] = o[n][d][0] * vmul;
-          dst[d * 16 + 8] = o[n][d][2] * vmul;
-          dst[D + d * 16] = o[n][d][1] * vmul;
-          dst[D + d * 16 + 8] = o[n][d][3] * vmul;
+          dst[d * 16] = o[n][d][0];
+          dst[d * 16 + 8] = o[n][d][2];
+          dst[D + d * 16] = o[n][d][1];
+          dst[D + d * 16 + 8] = o[n][d][3];
         }
         if (g == 0) {
-          wk.part_ml[slot * HT + h0] = make_float2(m[n][0], l0);
-          wk.part_ml[slot * HT + h0 + 1] = make_float2(m[n][1], l1);
+          wk.part_ml[slot * HT + h0] = make_float4(m[n][0], l0, lv_ref, 0.f);
+          wk.part_ml[slot * HT + h0 + 1] = make_float4(m[n][1], l1, lv_ref, 0.f);
         }
       }
     }
@@ -678,7 +677,8 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
 
 // Joins the parts of the runs that share boundaries cut, in the order of the keys.  One warp per
 // (share, column): the share that a cut run starts in describes it.  The parts' maxima and sums are
-// read by the lanes together, their O rows (4 dims per lane) eight at a time.
+// read by the lanes together, their O rows (4 dims per lane) eight at a time.  The sums are brought to
+// the first part's vs; the two factors are applied one after the other, since each alone fits 2^+-100.
 template <bool LIST, int NT>
 __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const Work wk) {
   constexpr int HT = 8 * NT;
@@ -697,14 +697,15 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const Work 
   for (int k = lane; k < cut.parts; k += 32) m = fmaxf(m, wk.part_ml[row_of(k)].x);
   m = warp_max(m);
   const float safe = m == -INFINITY ? 0.f : m;
+  const float lv_ref = wk.part_ml[row_of(0)].z;
   float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
   for (int k0 = 0; k0 < cut.parts; k0 += 32) {
     const int n = min(32, cut.parts - k0);
     float f = 0.f;
     if (lane < n) {
-      const float2 ml = wk.part_ml[row_of(k0 + lane)];
+      const float4 ml = wk.part_ml[row_of(k0 + lane)];
       f = ex2(ml.x - safe);
-      l += ml.y * f;
+      l += ml.y * f * ex2(fminf(lv_ref - ml.z, VS_SPREAD));
     }
     for (int k = 0; k < n; k += 8) {
       float4 v[8];
@@ -726,12 +727,13 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const Work 
     }
   }
   l = warp_sum(l);
-  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const float inv = l != 0.f ? 1.f / l : 0.f, v_ref = ex2(lv_ref);
   const int tok = LIST ? (cut.row + col) / a.group : 0;
   const int head = cut.kvh * a.group + (LIST ? (cut.row + col) % a.group : cut.row + col);
   *reinterpret_cast<uint2*>(a.out + (cut.q0 + tok) * a.out_ld + static_cast<int64_t>(head) * D +
                             lane * 4) =
-      make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+      make_uint2(pack_bf16x2(o[0] * inv * v_ref, o[1] * inv * v_ref),
+                 pack_bf16x2(o[2] * inv * v_ref, o[3] * inv * v_ref));
 }
 
 // Upper bound of the line's length.
@@ -760,12 +762,12 @@ void launch(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const a
   const int grid = static_cast<int>(
       std::max<int64_t>(1, std::min<int64_t>(148 * per_sm, (tiles + WARPS - 1) / WARPS)));
   wk.workers = grid * WARPS;
-  static_assert(sizeof(Cut) % 8 == 0, "the partials follow the cuts");
+  static_assert(sizeof(Cut) % 8 == 0, "the cuts follow the partials");
   const int64_t part_rows = static_cast<int64_t>(wk.workers) * 2 * HT;
-  at::Tensor ws = at::empty({wk.workers * static_cast<int64_t>(sizeof(Cut) / 4) + part_rows * (D + 2)},
+  at::Tensor ws = at::empty({wk.workers * static_cast<int64_t>(sizeof(Cut) / 4) + part_rows * (D + 4)},
                             like.options().dtype(at::kFloat));
   wk.part_o = ws.data_ptr<float>();
-  wk.part_ml = reinterpret_cast<float2*>(wk.part_o + part_rows * D);
+  wk.part_ml = reinterpret_cast<float4*>(wk.part_o + part_rows * D);
   wk.cut = reinterpret_cast<Cut*>(wk.part_ml + part_rows);
   auto rk = rows_kernel<LIST, NT>;
   auto jk = join_kernel<LIST, NT>;
