@@ -21,7 +21,8 @@
 //               unscaled: e4m3 is exact in f16, so the conversion is one cvt per pair, and rows past
 //               the sequence's end become zeros.
 //   warps 8-15  softmax, one thread per query row: it reads its row of q once (as f16, scaled by a
-//               power of two, into shared memory), then per tile 128 scores from TMEM.  ks of a
+//               power of two and with the softmax scale's sign, into shared memory), then per tile 128
+//               scores from TMEM.  ks of a
 //               16-key slice multiplies its scores, vs goes into the exponent:
 //                 P = 2^(s + log2 vs - m' + 7),  m' >= max(s + log2 vs) - 8,
 //               so P is at most 2^15 and keeps f16's 11 bits down to 2^-21 of the largest
@@ -66,6 +67,9 @@ constexpr int SMEM_BAR = SMEM_C + CST * NSL * 16;
 constexpr int SMEM_TOTAL = SMEM_BAR + 256 + 1024;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float LAZY = 8.f, SHIFT = 7.f;
+// Added to the factor of the raw scores (at most 2^31 of them in size), so that it is never zero: a masked
+// score is -inf, and -inf * 0 would be NaN.  Moves a score by less than 2^-94.
+constexpr float TINY = 1.17549435e-38f;   // 2^-126
 
 __device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t saddr, uint32_t lbo_bytes) {
   uint64_t d = 0;
@@ -462,8 +466,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       const int sh = q_shift(amax);
-      const float up = pow2i(sh);
-      row_scale = pow2i(-sh) * a.scale_log2;
+      // a negative softmax scale turns q's sign: row_scale stays positive, so the maximum of a slice's
+      // raw scores is that of its scaled ones
+      const float up = copysignf(pow2i(sh), a.scale_log2);
+      row_scale = pow2i(-sh) * fabsf(a.scale_log2);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -508,7 +514,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
       for (int i = 0; i < NSL; ++i) {
         const float4 v = cst[i];
-        sc[i] = v.x * row_scale;
+        sc[i] = fmaf(v.x, row_scale, TINY);
         lv[i] = v.y;
         vs0 = v.w;
       }

@@ -86,3 +86,19 @@ def test_v_scales_small_and_large(dev, form, exp):
     q = torch.randn(m * 3, 8, D, generator=torch.Generator().manual_seed(2)).bfloat16()
     out, ref, tol = _run(dev, form, (kc, vc, ks, vs, tables), lens, q)
     assert bool(((out - ref).abs() <= tol).all())
+
+
+@on_devices
+@on_forms
+@pytest.mark.parametrize("q_exp,k_exp,scale", [(-100, -40, None), (-20, -40, 1e-30), (0, 0, 0.0),
+                                               (0, 0, -0.1), (-100, -40, -1.0)])
+def test_scores_that_vanish_or_change_sign(dev, form, q_exp, k_exp, scale):
+    """A score factor (softmax scale, key scale, size of q) that underflows, is zero or negative:
+    masked keys stay masked."""
+    lens = [300, 75]
+    kc, vc, ks, vs, tables = _paged_inputs(lens, 2, 16, 5)
+    ks *= 2.0 ** k_exp
+    m, _ = FORMS[form]
+    q = torch.randn(m * 2, 8, D, generator=torch.Generator().manual_seed(3)) * 2.0 ** q_exp
+    out, ref, tol = _run(dev, form, (kc, vc, ks, vs, tables), lens, q.bfloat16(), scale)
+    assert bool(((out - ref).abs() <= tol).all())
