@@ -38,6 +38,7 @@ int64_t paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
                 op, ": q and out are bf16 [T, Hq, 128], contiguous heads, 16-byte aligned rows");
   TORCH_CHECK(q.sizes() == out.sizes(), op, ": out has q's shape");
   TORCH_CHECK(group >= 1 && q.size(1) == group * k_cache.size(1), op, ": Hq = group * Hkv");
+  TORCH_CHECK(q.size(0) * group < (int64_t(1) << 31) - 256, op, ": query rows exceed int32");
   const int64_t B = seq_lens.numel();
   TORCH_CHECK(block_tables.is_cuda() && block_tables.scalar_type() == at::kInt &&
                   block_tables.dim() == 2 && block_tables.size(0) >= B &&

@@ -236,8 +236,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   pdl_wait();
 
   const int seq = a.tile_seq[blockIdx.x];
-  const int row0 = a.tile_row0[blockIdx.x];
-  const bool bad = seq >= a.num_seqs || row0 < 0;
+  const int item_row0 = a.tile_row0[blockIdx.x];
+  const bool bad = seq >= a.num_seqs || item_row0 < 0;
   const bool used = seq >= 0 && !bad;
   if (bad && threadIdx.x == 0) record_error(a.err, kErrBounds);
   const int q_start = used ? a.cu_q[seq] : 0;
@@ -253,6 +253,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     kv_len = static_cast<int>(cap);
   }
   const int nrows_seq = q_len * a.group;
+  // an item past the sequence's rows has none; row0 + BM below must not pass 2^31
+  const int row0 = min(item_row0, nrows_seq);
   const int nqt = row0 + 128 < nrows_seq ? QT : 1;
   const int* btab = a.tables + (used ? seq * a.bt_stride : 0);
   // keys this CTA needs: causal rows see keys <= kv_len - q_len + token
