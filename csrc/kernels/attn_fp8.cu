@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include "attn_fp8.cuh"
+#include "checks.h"
 
 namespace lb {
 
@@ -29,6 +30,10 @@ int64_t paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   using namespace fp8a;
   const char* op = "paged_attention_fp8";
   check_fp8_cache(op, k_cache, v_cache, k_scale, v_scale);
+  const bool list = !decode && cu_q.has_value() && tile_seq.has_value() && tile_row0.has_value();
+  TORCH_CHECK(decode || list, op, ": prefill needs cu_q and the work list (tile_seq, tile_row0)");
+  check_same_device(op, k_cache, {&q, &out, &block_tables, &seq_lens, &err, list ? &*cu_q : nullptr,
+                                  list ? &*tile_seq : nullptr, list ? &*tile_row0 : nullptr});
   const c10::cuda::CUDAGuard guard(k_cache.device());
   for (const at::Tensor* t : {&q, (const at::Tensor*)&out})
     TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kBFloat16 && t->dim() == 3 &&
@@ -84,8 +89,6 @@ int64_t paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
     fp8_rows(a, false, group, tk, tv, q, st);
     return 2;
   }
-  TORCH_CHECK(cu_q.has_value() && tile_seq.has_value() && tile_row0.has_value(), op,
-              ": prefill needs cu_q and the work list (tile_seq, tile_row0)");
   for (const at::Tensor* t : {&*cu_q, &*tile_seq, &*tile_row0})
     TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kInt && t->is_contiguous(), op,
                 ": cu_q and the work list are contiguous int32");

@@ -22,6 +22,7 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include "checks.h"
 #include "common.cuh"
 
 namespace lb {
@@ -433,6 +434,7 @@ void check_fp8_cache(const char* op, const at::Tensor& k_cache, const at::Tensor
                   k_cache.is_contiguous() && v_cache.is_contiguous() &&
                   k_cache.sizes() == v_cache.sizes() && k_cache.size(3) == 128,
               op, ": caches are contiguous float8_e4m3fn [num_blocks, Hkv, block size, 128]");
+  check_same_device(op, k_cache, {&v_cache, &k_scale, &v_scale});
   const int64_t bs = k_cache.size(2);
   TORCH_CHECK(bs == 16 || bs == 32 || bs == 64, op, ": block size 16, 32 or 64");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(k_cache.data_ptr()) % 16 == 0 &&
@@ -456,6 +458,11 @@ at::Tensor rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const
                        at::Tensor& err) {
   using namespace kq;
   check_fp8_cache("rope_kv_fp8", k_cache, v_cache, k_scale, v_scale);
+  auto given = [](const c10::optional<at::Tensor>& t) {
+    return t.has_value() && t->defined() ? &*t : nullptr;
+  };
+  check_same_device("rope_kv_fp8", k_cache, {&qkv, &positions, &slots, &cos_sin, &err, given(out),
+                                             given(q_norm), given(k_norm)});
   const c10::cuda::CUDAGuard guard(k_cache.device());
   const int64_t T = qkv.size(0), R = cos_sin.size(1);
   TORCH_CHECK(hq >= 1 && hkv >= 1 && k_cache.size(1) == hkv, "rope_kv_fp8: head counts");

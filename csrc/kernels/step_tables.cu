@@ -24,6 +24,7 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include "checks.h"
 #include "common.cuh"
 
 namespace lb {
@@ -225,9 +226,11 @@ std::vector<at::Tensor> step_tables(const at::Tensor& ctx_lens, const at::Tensor
   TORCH_CHECK(seq_tables.is_cuda() && seq_tables.scalar_type() == at::kInt &&
                   seq_tables.dim() == 2 && (seq_tables.size(1) <= 1 || seq_tables.stride(1) == 1),
               "step_tables: seq_tables [S, W] int32, contiguous rows");
+  const bool has_rows = rows.has_value() && rows->defined();
+  check_same_device("step_tables", ctx_lens, {&q_lens, has_rows ? &*rows : nullptr, &seq_tables,
+                                              &new_blocks, &err});
   const c10::cuda::CUDAGuard guard(ctx_lens.device());
   const int64_t W = seq_tables.size(1);
-  const bool has_rows = rows.has_value() && rows->defined();
   if (has_rows)
     TORCH_CHECK(rows->is_cuda() && rows->scalar_type() == at::kInt && rows->is_contiguous() &&
                     rows->numel() == B,
