@@ -26,7 +26,7 @@ int64_t paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
                             const c10::optional<at::Tensor>& cu_q,
                             const c10::optional<at::Tensor>& tile_seq,
                             const c10::optional<at::Tensor>& tile_row0, int64_t group, double scale,
-                            bool decode, bool causal, at::Tensor& err) {
+                            bool decode, bool causal, int64_t item_rows, at::Tensor& err) {
   using namespace fp8a;
   const char* op = "paged_attention_fp8";
   check_fp8_cache(op, k_cache, v_cache, k_scale, v_scale);
@@ -98,13 +98,16 @@ int64_t paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   a.tile_seq = tile_seq->data_ptr<int>();
   a.tile_row0 = tile_row0->data_ptr<int>();
   a.num_tiles = tile_seq->numel();
-  // At most FEW_ROWS query rows per item on average (verification of a few tokens, tails of prompts):
-  // 256-row tiles would be mostly padding.  rows / tcgen05 kernel, us: 32 rows 64 x 4000 keys 196 / 278,
-  // 32 x 1280 49 / 52; 48 rows 32 x 1280 64 / 52; 64 rows 81 / 52.
+  // At most FEW_ROWS query rows per item (verification of a few tokens, tails of prompts): 256-row tiles
+  // would be mostly padding.  rows / tcgen05 kernel, us: 32 rows 64 x 4000 keys 196 / 278, 32 x 1280
+  // 49 / 52; 48 rows 32 x 1280 64 / 52; 64 rows 81 / 52.  The caller says how many rows its longest item
+  // has; a full item on the first kernel reads its keys 16 times (a 2048-token chunk over 16k beside 255
+  // decodes 2999 us instead of 675).  Else the mean decides, over all of q and all entries.
   constexpr int64_t FEW_ROWS = 32;
-  const int64_t avg = (q.size(0) * group + a.num_tiles - 1) / a.num_tiles;
-  if (avg <= FEW_ROWS && fp8_rows_fits(a, true)) {
-    fp8_rows(a, true, avg, tk, tv, q, st);
+  const int64_t rows_of_item =
+      item_rows > 0 ? item_rows : (q.size(0) * group + a.num_tiles - 1) / a.num_tiles;
+  if (rows_of_item <= FEW_ROWS && fp8_rows_fits(a, true)) {
+    fp8_rows(a, true, rows_of_item, tk, tv, q, st);
     return 2;
   }
   fp8_prefill(a, tk, tv, st);

@@ -100,7 +100,7 @@ __device__ __forceinline__ int checked_block(const Args& a, int id) {
 // fp8_rows (attn_fp8_rows.cu): few query rows per sequence, one token each (list = false) or the
 // work list's.  fp8_prefill (attn_fp8_prefill.cu): the work list's 256-row items on tcgen05.
 bool fp8_rows_fits(const fp8a::Args& a, bool list);
-// rows: a work list's query rows per item, on average.
+// rows: query rows of a work list's longest item (or their mean, where only that is known).
 void fp8_rows(const fp8a::Args& a, bool list, int64_t rows, const CUtensorMap& tk,
               const CUtensorMap& tv, const at::Tensor& like, cudaStream_t st);
 void fp8_prefill(const fp8a::Args& a, const CUtensorMap& tk, const CUtensorMap& tv,

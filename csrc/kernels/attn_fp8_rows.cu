@@ -789,8 +789,8 @@ bool fp8_rows_fits(const fp8a::Args& a, bool list) {
 void fp8_rows(const fp8a::Args& a, bool list, int64_t rows, const CUtensorMap& tk,
               const CUtensorMap& tv, const at::Tensor& like, cudaStream_t st) {
   using namespace fp8d;
-  // As many column tiles as hold a decode group (16 columns at a time beyond that), or a list's items
-  // on average, so that one pass over the keys does.  Lists of 64 items over 4000 keys, us with 1 / 2 /
+  // As many column tiles as hold a decode group (16 columns at a time beyond that), or a list's items,
+  // so that one pass over the keys does.  Lists of 64 items over 4000 keys, us with 1 / 2 /
   // 3 column tiles: 8 rows 94 / 105 / 139, 12 rows 178 / 107 / 140, 20 rows 266 / 192 / 143, 32 rows
   // 351 / 196 / 257 (two passes of 16 beat 24 + 8).
   if (list && (rows > 24 || (rows > 8 && rows <= 16))) launch<true, 2>(a, tk, tv, like, st);

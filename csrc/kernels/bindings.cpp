@@ -109,7 +109,7 @@ int64_t paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
                             const c10::optional<at::Tensor>& cu_q,
                             const c10::optional<at::Tensor>& tile_seq,
                             const c10::optional<at::Tensor>& tile_row0, int64_t group, double scale,
-                            bool decode, bool causal, at::Tensor& err);
+                            bool decode, bool causal, int64_t item_rows, at::Tensor& err);
 }  // namespace lb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

@@ -501,7 +501,9 @@ class ModelRunner:
                                  self.block_size, group=self.model.group, num_decode=num_decode)
             d_pos, d_slots, d_bt = st.positions, st.slots, st.block_tables
             d_seq_lens, d_cu_q = st.seq_lens, st.cu_q
-            tiles = (st.tile_seq, st.tile_row0) if num_decode < B else None
+            # the list has a spare entry per request: pass on those in use
+            n_items, item_rows = ops.work_items(q_lens[num_decode:], self.model.group)
+            tiles = (st.tile_seq[:n_items], st.tile_row0[:n_items]) if n_items else None
         else:
             d_bt = dtake(B * width).view(B, width)
             cu_list = cu_q.tolist()
@@ -509,6 +511,7 @@ class ModelRunner:
                                    block_size=self.block_size, head_dim=self.model.d)
             tiles = torch.tensor([ts, tr], dtype=torch.int32).to(self.device, non_blocking=True) \
                 if ts else None
+            item_rows = 0
         if fwd:
             ops.forward_tokens(d_ids[:num_decode], d_src, self.d_last_out)
         max_len = int(seq_lens.max()) if B else 1
@@ -516,6 +519,7 @@ class ModelRunner:
                           num_decode=num_decode,
                           tile_seq=tiles[0] if tiles is not None else None,
                           tile_row0=tiles[1] if tiles is not None else None,
+                          item_rows=item_rows,
                           decode_splits=ops.decode_splits(num_decode, self.model.hkv, max_len)
                           if self.is_cuda and not fp8 else 1,
                           seq_lens_cpu=torch.from_numpy(seq_lens.copy()),

@@ -103,6 +103,7 @@ class ForwardBatch:
     num_decode: int              # first num_decode sequences have exactly one query token
     tile_seq: Optional[torch.Tensor] = None    # prefill attention work list
     tile_row0: Optional[torch.Tensor] = None
+    item_rows: int = 0                         # query rows of its longest item (8-bit KV cache)
     decode_splits: int = 1
     seq_lens_cpu: Optional[torch.Tensor] = None
     cu_q_cpu: Optional[torch.Tensor] = None
@@ -295,7 +296,8 @@ class LlamaModel:
             if tiles:
                 ops.paged_attention_fp8(q, *cache, b.block_tables, b.seq_lens, b.cu_q, out,
                                         self.group, decode=False, tile_seq=b.tile_seq,
-                                        tile_row0=b.tile_row0, scale=self.scale)
+                                        tile_row0=b.tile_row0, scale=self.scale,
+                                        item_rows=b.item_rows)
             return q
         self._rope_kv(qkv, b, kv, i, L)
         q = qkv[:, :self.hq * self.d].view(T, self.hq, self.d)

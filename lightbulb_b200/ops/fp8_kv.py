@@ -8,13 +8,15 @@ together::
 
     t = ops.step_tables(ctx_lens, q_lens, rows, seq_tables, new_blocks, T, block_size, ...)
     q = ops.rope_kv_fp8(qkv, t.positions, t.slots, cos_sin, k, v, k_scale, v_scale, hq, hkv)
+    n, most = ops.work_items(host_q_lens, group)      # entries in use, rows of the longest
     ops.paged_attention_fp8(q, k, v, k_scale, v_scale, t.block_tables, t.seq_lens, t.cu_q, out,
-                            group, decode, tile_seq=t.tile_seq, tile_row0=t.tile_row0)
+                            group, decode, tile_seq=t.tile_seq[:n], tile_row0=t.tile_row0[:n],
+                            item_rows=most)
 """
 from __future__ import annotations
 
 import math
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -35,6 +37,15 @@ def _err(t: torch.Tensor) -> torch.Tensor:
     if w is None:
         w = _err_words[i] = scratch(t.device).err
     return w
+
+
+def work_items(q_lens: Sequence[int], group: int, rows_per_tile: int = 256) -> Tuple[int, int]:
+    """Of the work list that :func:`step_tables` builds for requests with ``q_lens`` new tokens (those
+    from ``num_decode`` on): how many entries are in use, all in front, and the query rows of the
+    longest."""
+    rows = [int(n) * group for n in q_lens]
+    return (sum(-(-r // rows_per_tile) for r in rows),
+            min(max(rows, default=0), rows_per_tile))
 
 
 class StepTables(NamedTuple):
@@ -183,7 +194,7 @@ def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                         cu_q: Optional[torch.Tensor], out: torch.Tensor, group: int,
                         decode: bool, tile_seq: Optional[torch.Tensor] = None,
                         tile_row0: Optional[torch.Tensor] = None, causal: bool = True,
-                        scale: Optional[float] = None) -> torch.Tensor:
+                        scale: Optional[float] = None, item_rows: int = 0) -> torch.Tensor:
     """Attention over the 8-bit cache; q, out [T, Hq, 128] bf16 (rows may be strided).
 
     ``decode``: token i belongs to sequence i and sees its ``seq_lens[i]`` keys.  Otherwise
@@ -191,14 +202,21 @@ def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     (``tile_seq``, ``tile_row0``: one entry per 256 packed rows, -1 entries skipped) says which
     sequences are computed; with ``causal`` a token sees the keys up to its own.  Rows without a
     visible key give 0.  ``scale`` defaults to 1 / sqrt(128) (pass 1 / sqrt(true head_dim) for
-    zero-padded heads)."""
+    zero-padded heads).
+
+    ``item_rows``: query rows (tokens times ``group``) of the work list's longest item, which decides
+    the kernel; results do not depend on it but for rounding.  0: the mean of q's rows over the list's
+    entries stands in for it, so a list with many -1 entries, or a q with many rows that are not the
+    list's, should come with the number (:func:`work_items`)."""
     d = q.shape[-1]
     if scale is None:
         scale = 1.0 / math.sqrt(d)
+    if item_rows < 0:
+        raise ValueError(f"paged_attention_fp8: item_rows {item_rows}")
     if q.is_cuda:
         _launches[0] += _need_c().paged_attention_fp8(
             q, k_cache, v_cache, k_scale, v_scale, out, block_tables, seq_lens, cu_q, tile_seq,
-            tile_row0, group, scale, decode, causal, _err(q))
+            tile_row0, group, scale, decode, causal, item_rows, _err(q))
         return out
     # CPU restatement
     from ..models.reference import attention_ref

@@ -28,3 +28,70 @@ def test_items_past_the_rows_write_nothing(dev, m, row0):
     ref, tol = _attention_ref(q, kc, vc, ks, vs, tables, lens, [m], group, True, None)
     assert bool(((out.cpu().double() - ref).abs() <= tol).all())
     assert bool((buf[:32] == 3).all()) and bool((buf[32 + m:] == 3).all())
+
+
+MIXED = [  # decodes, new tokens of each other request, group, kernels of the list's call
+    (63, [70], 4, 1), (40, [130, 3], 1, 1), (255, [600], 4, 1), (30, [5, 4], 4, 2), (0, [40], 8, 1)]
+
+
+@on_devices
+@pytest.mark.parametrize("nd,chunks,group,kernels", MIXED)
+def test_prompt_chunks_beside_decodes(dev, nd, chunks, group, kernels):
+    """A step as the engine runs it: decodes first, their tokens in the same q, the list of
+    step_tables.  The chunks' rows decide the kernel, however many decodes the step has."""
+    gen = torch.Generator().manual_seed(nd + group)
+    n_q = [1] * nd + chunks
+    lens = [int(torch.randint(1, 90, (1,), generator=gen)) for _ in range(nd)] + \
+        [n + 37 for n in chunks]
+    kc, vc, ks, vs, tables = _paged_inputs(lens, 2, 16, nd)
+    args = [z.to(dev) for z in (kc, vc, ks, vs)]
+    t, hq, b = sum(n_q), 2 * group, len(n_q)
+    st = ops.step_tables(_i32([n - m for n, m in zip(lens, n_q)], dev), _i32(n_q, dev), None,
+                         _i32(tables, dev), _i32([0] * (t + b), dev), t, 16, group=group,
+                         num_decode=nd)
+    tab = _i32(tables, dev)             # the blocks that hold the tokens already
+    q = torch.randn(t, hq, D, generator=gen).bfloat16()
+    out = torch.full((t, hq, D), 7.0, dtype=torch.bfloat16, device=dev)
+    qd = q.to(dev)
+    if nd:
+        ops.paged_attention_fp8(qd, *args, tab[:nd], st.seq_lens[:nd], None, out, group, True)
+    n, most = ops.work_items(chunks, group)
+    assert most == min(256, max(chunks) * group)
+    assert (st.tile_seq >= 0).tolist() == [True] * n + [False] * (st.tile_seq.numel() - n)
+    bits = []
+    for k in (n, st.tile_seq.numel()):  # entries in use alone, and with the spare ones
+        n0 = ops.launch_counter_value()
+        ops.paged_attention_fp8(qd, *args, tab, st.seq_lens, st.cu_q, out, group, False,
+                                tile_seq=st.tile_seq[:k], tile_row0=st.tile_row0[:k],
+                                item_rows=most)
+        if dev == "cuda":
+            assert ops.launch_counter_value() - n0 == kernels
+            torch.cuda.synchronize()
+            ops.check_errors()
+        bits.append(out.cpu().clone())
+    assert torch.equal(*bits)
+    ref, tol = _attention_ref(q, kc, vc, ks, vs, tables, lens, n_q, group, True, None)
+    assert bool(((bits[0].double() - ref).abs() <= tol).all())
+
+
+def test_engine_passes_the_items_in_use(monkeypatch):
+    """Every list that reaches the attention has only real entries and says how long the longest
+    is, also with more decodes than chunks."""
+    from test_kv_fp8_engine import GREEDY, _engine
+    _, _, _, eng = _engine("cpu", overlap=False)
+    calls, inner = [], ops.paged_attention_fp8
+
+    def watch(q, *a, **k):
+        if not k["decode"]:
+            seq, row0, cu = k["tile_seq"].tolist(), k["tile_row0"].tolist(), a[6].tolist()
+            rows = [(cu[s + 1] - cu[s]) * eng.model.group for s in seq]
+            assert min(seq) >= 0 and all(r < n for r, n in zip(row0, rows))
+            assert k["item_rows"] == min(256, max(rows))
+            calls.append((q.shape[0], sum(set(rows))))
+        return inner(q, *a, **k)
+    monkeypatch.setattr(ops, "paged_attention_fp8", watch)
+    prompts = [[i + 1, 2, 3] for i in range(7)] + [list(range(200))]
+    eng.generate(prompt_token_ids=prompts, params=GREEDY)
+    assert any(t * eng.model.group > r for t, r in calls)      # steps with decodes and chunks
+    with pytest.raises(ValueError):
+        inner(torch.zeros(1, 1, D), *[None] * 8, 1, False, item_rows=-1)
