@@ -258,14 +258,16 @@ class SpeculativeDecoder:
 def attach_speculative(engine, draft_model, draft_cfg, k: int = 4, num_blocks: int = 0,
                        use_cuda_graphs: bool = True, min_acceptance: float = 0.3,
                        fallback_after: int = 10) -> SpeculativeDecoder:
-    """Give ``engine`` a draft model (a ``LlamaModel`` with the same tokenizer)."""
+    """Give ``engine`` a draft model (a ``LlamaModel`` with the same tokenizer).  The draft's KV pool
+    has the elements of the engine's and, by default, half its blocks."""
     from ..kv.block_manager import BlockManager
     from ..models.llama import KVCache
     from .model_runner import ModelRunner
     c = engine.cfg
     nb = num_blocks or max(64, engine.blocks.num_blocks // 2)
     kv = KVCache(draft_cfg.num_layers, nb, draft_model.hkv, c.cache.block_size,
-                 draft_cfg.head_dim_padded, device=draft_model.device)
+                 draft_cfg.head_dim_padded, dtype=engine.kv.storage.dtype,
+                 device=draft_model.device)
     dbm = BlockManager(nb, c.cache.block_size, enable_prefix=False)
     runner = ModelRunner(draft_model, kv, dbm, c.scheduler.max_num_seqs,
                          c.scheduler.max_num_batched_tokens + c.scheduler.max_num_seqs * (k + 1),

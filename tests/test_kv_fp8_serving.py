@@ -1,0 +1,34 @@
+"""What the engine generates from the 8-bit cache, token by token against the fp32 oracle."""
+import pytest
+import torch
+
+from lightbulb_b200.models.reference import ReferenceLlama
+from test_kv_fp8_engine import GREEDY, PROMPTS, _check, _engine, _watch_slots, on_devices
+
+
+def _check_tokens(cfg, w, prompts, outs):
+    """Every emitted token's oracle logit lies within half a standard deviation of its row's best.
+    (The cache's elements are off by up to 2^-4 of their value; a token picked at random lies about
+    four deviations below the best of a vocabulary of this size.)"""
+    ref = ReferenceLlama(cfg, w)
+    for p, out in zip(prompts, outs):
+        ref.reset()
+        lg = ref.forward(torch.tensor(p + out[:-1]))[len(p) - 1:]
+        for row, t in zip(lg, out):
+            assert float(row.max() - row[t]) <= 0.5 * float(row.std())
+
+
+@on_devices
+def test_the_draft_has_the_engines_cache(dev):
+    """The draft's pool is 8-bit too: as many blocks, half the bytes of a bf16 one.  With the
+    target's own weights nearly every proposal is accepted, and what is emitted is right."""
+    cfg, w, packed, eng = _engine(dev)
+    spec = eng.attach_draft(packed, cfg, k=3)
+    kv = spec.draft.kv
+    assert kv.storage.dtype == eng.kv.storage.dtype and kv.num_blocks == eng.kv.num_blocks
+    assert kv.storage.numel() * kv.storage.element_size() == eng.kv.storage.numel()
+    _watch_slots(eng)
+    outs = [s.output_token_ids for s in eng.generate(prompt_token_ids=PROMPTS, params=GREEDY)]
+    _check(dev)
+    assert spec.stats.rounds > 0 and spec.stats.acceptance_rate() > 0.7
+    _check_tokens(cfg, w, PROMPTS, outs)
