@@ -2,6 +2,9 @@
 #pragma once
 
 #include <ATen/core/Tensor.h>
+#include <c10/cuda/CUDAException.h>
+
+#include <atomic>
 
 #include "common.cuh"
 
@@ -75,13 +78,15 @@ __device__ __forceinline__ int q_shift(float amax) {
 }
 __device__ __forceinline__ float pow2i(int k) { return __uint_as_float((k + 127) << 23); }
 
-// cudaFuncSetAttribute holds for one device: true the first time on the current one.
-inline bool first_on_device(bool (&done)[64]) {
+// Lets the kernel have `bytes` of dynamic shared memory on the current device, once per device.  `done` is
+// set only after the attribute holds: no other host thread launches before, and a failure is tried again.
+template <typename K>
+inline void allow_smem(K* kernel, int bytes, std::atomic<bool> (&done)[64]) {
   int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 64 && done[dev]) return false;
-  if (dev < 64) done[dev] = true;
-  return true;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 64 && done[dev].load(std::memory_order_acquire)) return;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done[dev].store(true, std::memory_order_release);
 }
 
 // Physical block of slice `s` (16 keys) of a sequence; an id outside the pool is reported and

@@ -680,10 +680,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 void fp8_prefill(const fp8a::Args& a, const CUtensorMap& tk, const CUtensorMap& tv,
                  cudaStream_t st) {
   using namespace fp8p;
-  static bool attr[64] = {};
-  if (first_on_device(attr))
-    C10_CUDA_CHECK(cudaFuncSetAttribute(prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        SMEM_TOTAL));
+  static std::atomic<bool> allowed[64] = {};
+  allow_smem(prefill_kernel, SMEM_TOTAL, allowed);
   C10_CUDA_CHECK(launch_k(prefill_kernel, dim3(a.num_tiles, a.hkv), dim3(THREADS), SMEM_TOTAL, st,
                           nullptr, 0, tk, tv, a));
 }

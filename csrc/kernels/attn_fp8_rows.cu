@@ -751,10 +751,8 @@ void launch(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const a
   wk.entries = LIST ? a.num_tiles : a.num_seqs;
   const size_t lens = 2 * WARPS * sizeof(int) + Entries<LIST>::bytes(wk.entries);
   const size_t smem = 1024 + WARPS * (WARP_SMEM + q_smem_of(NT)) + WARPS * STAGES * 24 + lens;
-  static bool attr[64] = {};
-  if (first_on_device(attr))
-    C10_CUDA_CHECK(cudaFuncSetAttribute(rows_kernel<LIST, NT>,
-                                        cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+  static std::atomic<bool> allowed[64] = {};
+  allow_smem(rows_kernel<LIST, NT>, 227 * 1024, allowed);
   // fewer CTAs an SM when the entries' tables of a very large batch need the room; no more warps
   // than the tiles there can be make shares
   const int per_sm = std::max<int>(1, std::min<size_t>(ctas_of(NT), 228 * 1024 / (smem + 1024)));
