@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* s_free = s_full + QT;          // S of a slot in registers (4 softmax warps)
   uint64_t* p_ready = s_free + 1;          // [QT] P_t in TMEM (4 softmax warps)
   uint64_t* pv_done = p_ready + QT;        // [QT] P_t V
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + QT);
+  uint64_t* mma_drain = pv_done + QT;      // every MMA issued, after an abort
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -211,6 +212,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&c_empty[s], 8);
     }
     mbar_init(s_free, 4);
+    mbar_init(mma_drain, 1);
     for (int t = 0; t < QT; ++t) {
       mbar_init(&s_full[t], 1);
       mbar_init(&p_ready[t], 4);
@@ -351,6 +353,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!ok) {
         if (lane == 0) record_error(a.err, kErrTimeoutTmaFull);
         *abort_flag = 1;
+        // MMAs still in flight read shared memory and write TMEM: no exit before they are done
+        commit_if(leader, mma_drain);
+        if (!mbar_wait(mma_drain, 0, nullptr) && lane == 0) record_error(a.err, kErrTimeoutDrain);
       }
     } else if (warp == 2 && ntiles > 0) {
       // slice constants, vs relative to the first slice's vs0: ks, log2(vs / vs0), vs0 / vs, vs0
