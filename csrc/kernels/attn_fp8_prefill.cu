@@ -353,9 +353,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!ok) {
         if (lane == 0) record_error(a.err, kErrTimeoutTmaFull);
         *abort_flag = 1;
-        // MMAs still in flight read shared memory and write TMEM: no exit before they are done
-        commit_if(leader, mma_drain);
-        if (!mbar_wait(mma_drain, 0, nullptr) && lane == 0) record_error(a.err, kErrTimeoutDrain);
       }
     } else if (warp == 2 && ntiles > 0) {
       // slice constants, vs relative to the first slice's vs0: ks, log2(vs / vs0), vs0 / vs, vs0
@@ -663,8 +660,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   }
 
-  // after an abort: wait (bounded) for this CTA's TMA copies still in flight
+  // after an abort: wait (bounded) for this CTA's MMAs and TMA copies still in flight
   __syncthreads();
+  if (warp == 1 && *abort_flag) {
+    commit_if(elect_one(), mma_drain);         // of the lane that issued the MMAs
+    if (!mbar_wait(mma_drain, 0, nullptr) && lane == 0) record_error(a.err, kErrTimeoutDrain);
+  }
   if (warp == 0 && lane == 0 && *abort_flag) {
     bool drained = true;
     for (int s = 0; s < SST; ++s)
