@@ -191,8 +191,9 @@ class CacheConfig:
     num_blocks: int = 0  # 0 -> derive from free memory
     gpu_memory_utilization: float = 0.90
     enable_prefix_caching: bool = True
-    # "bf16", or "fp8": e4m3 with one scale per block of tokens and KV head (half the bytes; block
-    # size 16, 32 or 64; not with KV compression, the segmented cache or saved KV rows)
+    # "bf16" (also spelt "bfloat16" or "auto"), or "fp8": e4m3 with one scale per block of tokens
+    # and KV head (half the bytes; block size 16, 32 or 64; not with KV compression, the segmented
+    # cache or saved KV rows).  Pipeline parallelism has its own bf16 cache.
     kv_dtype: str = "bf16"
     # KV compression (H2O heavy hitters / StreamingLLM sinks); 0 disables.
     h2o_budget: int = 0

@@ -27,7 +27,8 @@ from .. import ops
 from ..config import ModelConfig
 
 
-KV_DTYPES = {"bf16": torch.bfloat16, "fp8": ops.FP8_KV_DTYPE}
+KV_DTYPES = {"bf16": torch.bfloat16, "bfloat16": torch.bfloat16, "auto": torch.bfloat16,
+             "fp8": ops.FP8_KV_DTYPE}
 
 
 def kv_dtype_of(name: str) -> torch.dtype:

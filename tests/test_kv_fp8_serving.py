@@ -32,3 +32,10 @@ def test_the_draft_has_the_engines_cache(dev):
     _check(dev)
     assert spec.stats.rounds > 0 and spec.stats.acceptance_rate() > 0.7
     _check_tokens(cfg, w, PROMPTS, outs)
+
+
+@pytest.mark.parametrize("name", ["bf16", "bfloat16", "auto"])
+def test_names_of_the_bf16_cache(name):
+    """The field was not read once: configurations that spell bf16 otherwise still run."""
+    _, _, _, eng = _engine("cpu", kv_dtype=name, block_size=8)
+    assert eng.kv.storage.dtype == torch.bfloat16 and not eng.kv.fp8
