@@ -461,6 +461,11 @@ class ModelRunner:
         self._fill_block_tables([c.seq for c in chunks], bt, width)
         n_new = 0
         if fp8:
+            if B > len(self.tables.mirror):     # the scheduler's limit was raised meanwhile
+                if self.is_cuda:
+                    torch.cuda.synchronize()    # a step in flight still reads the old table
+                self.tables.grow(B + 8)
+                self.release_graphs()
             rows[:], new = self.tables.place([c.seq.seq_id for c in chunks], bt, ctx, q_lens,
                                              self.block_size)
             n_new = len(new)

@@ -24,6 +24,17 @@ class ResidentTables:
         self.free = list(range(rows - 1, -1, -1))
         self.uploads = 0                                       # rows uploaded so far
 
+    def grow(self, rows: int) -> None:
+        """Room for ``rows`` sequences in a step.  The device table moves: what was captured with
+        the old one has to be captured again."""
+        more = rows - len(self.mirror)
+        if more <= 0:
+            return
+        width = self.mirror.shape[1]
+        self.free += list(range(rows - 1, len(self.mirror) - 1, -1))
+        self.mirror = np.concatenate([self.mirror, np.zeros((more, width), np.int32)])
+        self.tables = torch.cat([self.tables, self.tables.new_zeros(more, width)])
+
     def _rows(self, seq_ids: List[int]) -> np.ndarray:
         batch = set(seq_ids)
         out = np.empty(len(seq_ids), dtype=np.int64)

@@ -39,3 +39,24 @@ def test_names_of_the_bf16_cache(name):
     """The field was not read once: configurations that spell bf16 otherwise still run."""
     _, _, _, eng = _engine("cpu", kv_dtype=name, block_size=8)
     assert eng.kv.storage.dtype == torch.bfloat16 and not eng.kv.fp8
+
+
+@on_devices
+@pytest.mark.parametrize("graphs", [False, True])
+def test_more_sequences_than_at_the_start(dev, graphs):
+    """The batch-size adjuster raises the scheduler's limit while the engine runs: steps with more
+    sequences than the resident tables have rows, and smaller ones (captured graphs) after them."""
+    if graphs and dev == "cpu":
+        pytest.skip("CUDA graphs")
+    cfg, w, _, eng = _engine(dev, num_blocks=200, graphs=graphs)
+    first = [s.output_token_ids for s in eng.generate(prompt_token_ids=PROMPTS, params=GREEDY)]
+    rows = eng.runner.tables.tables.shape[0]
+    n = rows + 5
+    eng.scheduler.cfg.max_num_seqs = n
+    prompts = [[i + 3, i, 2 * i] for i in range(n)]
+    outs = [s.output_token_ids for s in eng.generate(prompt_token_ids=prompts, params=GREEDY)]
+    again = [s.output_token_ids for s in eng.generate(prompt_token_ids=PROMPTS, params=GREEDY)]
+    _check(dev)
+    assert eng.runner.tables.tables.shape[0] >= n
+    assert eng.runner.tables.tables.cpu().tolist() == eng.runner.tables.mirror.tolist()
+    _check_tokens(cfg, w, PROMPTS + prompts + PROMPTS, first + outs + again)
