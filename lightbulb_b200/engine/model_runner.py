@@ -137,6 +137,9 @@ class ModelRunner:
         self.block_size = kv.block_size
         self.max_blocks_per_seq = (max_model_len + self.block_size - 1) // self.block_size + 1
         self.use_graphs = use_cuda_graphs and self.is_cuda
+        if kv.fp8 and max_num_seqs > ops.MAX_REQUESTS:
+            raise ValueError(f"kv_dtype='fp8': at most {ops.MAX_REQUESTS} sequences in a step, "
+                             f"max_num_seqs is {max_num_seqs}")
         self.tables = ResidentTables(max_num_seqs + 8, self.max_blocks_per_seq, self.device) \
             if kv.fp8 else None
         step = comm.world if (comm is not None and getattr(comm, "fused_requested", False)) else 1

@@ -428,5 +428,5 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
 # ------------------------------------------------------------------------------------
 # 8-bit paged KV cache
 # ------------------------------------------------------------------------------------
-from .fp8_kv import (FP8_KV_DTYPE, StepTables, paged_attention_fp8,  # noqa: E402,F401
-                     rope_kv_fp8, step_tables, work_items)
+from .fp8_kv import (FP8_KV_DTYPE, MAX_REQUESTS, StepTables,  # noqa: E402,F401
+                     paged_attention_fp8, rope_kv_fp8, step_tables, work_items)

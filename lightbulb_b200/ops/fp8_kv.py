@@ -25,6 +25,7 @@ from . import _launches, _need_c, scratch
 FP8_KV_DTYPE = torch.float8_e4m3fn
 FP8_MAX = 448.0                            # largest e4m3 value
 FP8_SCALE_MIN_EXP, FP8_SCALE_MAX_EXP = -40, 119
+MAX_REQUESTS = 4096                        # requests of a step, sequences of a decode call
 
 
 _err_words: dict = {}       # device index -> error word of its scratch
@@ -77,8 +78,8 @@ def step_tables(ctx_lens: torch.Tensor, q_lens: torch.Tensor, rows: Optional[tor
     outside ``seq_tables``, too few ``new_blocks`` or too few token rows are reported through
     the error word (:func:`check_errors`); what they concern gets slot -1."""
     b, w = ctx_lens.numel(), seq_tables.shape[1]
-    if not 1 <= b <= 4096:
-        raise ValueError(f"step_tables: {b} requests (1 to 4096)")
+    if not 1 <= b <= MAX_REQUESTS:
+        raise ValueError(f"step_tables: {b} requests (1 to {MAX_REQUESTS})")
     if num_tokens < 0 or group < 1 or rows_per_tile < 1:
         raise ValueError("step_tables: num_tokens, group, rows_per_tile")
     if block_size < 1 or block_size > 1024 or block_size & (block_size - 1):

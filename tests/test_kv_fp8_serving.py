@@ -2,6 +2,9 @@
 import pytest
 import torch
 
+from lightbulb_b200 import ops
+from lightbulb_b200.config import CacheConfig, EngineConfig, SchedulerConfig
+from lightbulb_b200.engine.llm_engine import LLMEngine
 from lightbulb_b200.models.reference import ReferenceLlama
 from test_kv_fp8_engine import GREEDY, PROMPTS, _check, _engine, _watch_slots, on_devices
 
@@ -60,3 +63,17 @@ def test_more_sequences_than_at_the_start(dev, graphs):
     assert eng.runner.tables.tables.shape[0] >= n
     assert eng.runner.tables.tables.cpu().tolist() == eng.runner.tables.mirror.tolist()
     _check_tokens(cfg, w, PROMPTS + prompts + PROMPTS, first + outs + again)
+
+
+def test_too_many_sequences_are_refused_when_the_engine_is_built():
+    """Not by the step that first has them."""
+    cfg, _, packed, _ = _engine("cpu")
+
+    def build(kv_dtype, n):
+        return LLMEngine(EngineConfig(model=cfg, cache=CacheConfig(num_blocks=16, kv_dtype=kv_dtype),
+                                      scheduler=SchedulerConfig(max_num_seqs=n, max_model_len=64,
+                                                                max_num_batched_tokens=64)), packed)
+    build("bf16", ops.MAX_REQUESTS + 1)
+    build("fp8", ops.MAX_REQUESTS)
+    with pytest.raises(ValueError, match="max_num_seqs"):
+        build("fp8", ops.MAX_REQUESTS + 1)
