@@ -293,7 +293,9 @@ def bench_decode(args):
     launches = ops.launch_counter_value()
     dev_ms = eng.runner.step_events_total_ms()
     eng.runner.disable_step_events()
-    clk = clocks.stop()
+    t_clk = time.perf_counter()
+    clk = clocks.stop()          # ends nvidia-smi: no part of the generation
+    clk_s = time.perf_counter() - t_clk
     ops.check_errors(dev)
     # ---- phase 4 (not part of the timed K steps): the rest of the generation, so the line
     # also carries decode throughput over every output token, not only the early window ----
@@ -303,7 +305,7 @@ def bench_decode(args):
     while eng.has_unfinished():
         gen_tokens += len(eng.step())
     gen_dev_ms += eng.runner.step_events_total_ms()
-    gen_wall = time.perf_counter() - gen_w0
+    gen_wall = time.perf_counter() - gen_w0 - clk_s
     eng.runner.disable_step_events()
     ops.check_errors(dev)
     if comm is not None:
