@@ -48,7 +48,7 @@ struct Args {
   const bf16* q_norm;
   const bf16* k_norm;
   float inv_norm_dim, eps;
-  int T, hq, hkv, bs, num_blocks;
+  int T, hq, hkv, num_blocks;
   int* err;
 };
 
@@ -516,7 +516,6 @@ at::Tensor rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const
   a.T = T;
   a.hq = hq;
   a.hkv = hkv;
-  a.bs = k_cache.size(2);
   a.num_blocks = k_cache.size(0);
   a.err = err.data_ptr<int>();
   // A warp per row (and head pair) while that leaves the GPU room: a decode batch, every row its own
@@ -529,9 +528,10 @@ at::Tensor rope_kv_fp8(const at::Tensor& qkv, const at::Tensor& positions, const
   const int64_t kv = few ? (T * pairs + WPC - 1) / WPC : (T + 15) / 16 * pairs;
   const int64_t qw = ((T + 1) / 2 * ((hq + HPW - 1) / HPW) + WPC - 1) / WPC;
   TORCH_CHECK(kv + qw < (int64_t(1) << 31), "rope_kv_fp8: too many rows");
-  auto kernel = a.bs == 16   ? (few ? rope_kv_fp8_kernel<16, 1> : rope_kv_fp8_kernel<16, 4>)
-                : a.bs == 32 ? (few ? rope_kv_fp8_kernel<32, 1> : rope_kv_fp8_kernel<32, 4>)
-                             : (few ? rope_kv_fp8_kernel<64, 1> : rope_kv_fp8_kernel<64, 4>);
+  const int64_t bs = k_cache.size(2);
+  auto kernel = bs == 16   ? (few ? rope_kv_fp8_kernel<16, 1> : rope_kv_fp8_kernel<16, 4>)
+                : bs == 32 ? (few ? rope_kv_fp8_kernel<32, 1> : rope_kv_fp8_kernel<32, 4>)
+                           : (few ? rope_kv_fp8_kernel<64, 1> : rope_kv_fp8_kernel<64, 4>);
   C10_CUDA_CHECK(launch_k(kernel, dim3(kv + qw), dim3(THREADS), 0,
                           at::cuda::getCurrentCUDAStream(), nullptr, 0, a, win,
                           static_cast<int>(kv)));
