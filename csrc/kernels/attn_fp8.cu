@@ -99,8 +99,8 @@ int64_t paged_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
   a.tile_row0 = tile_row0->data_ptr<int>();
   a.num_tiles = tile_seq->numel();
   // At most FEW_ROWS query rows per item (verification of a few tokens, tails of prompts): 256-row tiles
-  // would be mostly padding.  rows / tcgen05 kernel, us: 32 rows 64 x 4000 keys 196 / 278, 32 x 1280
-  // 49 / 52; 48 rows 32 x 1280 64 / 52; 64 rows 81 / 52.  The caller says how many rows its longest item
+  // would be mostly padding.  rows / tcgen05 kernel, us: 32 rows 64 x 4000 keys 193 / 311, 32 x 1280
+  // 48 / 58; 48 rows 32 x 1280 62 / 58; 64 rows 79 / 59.  The caller says how many rows its longest item
   // has; a full item on the first kernel reads its keys 16 times (a 2048-token chunk over 16k beside 255
   // decodes 2999 us instead of 675).  Else the mean decides, over all of q and all entries.
   constexpr int64_t FEW_ROWS = 32;

@@ -33,8 +33,9 @@
 // (40 + 72 + 200 + 200 = 4 * 128 per quarter).  Every wait is bounded; on expiry the kernel records an
 // error and unwinds.
 //
-// Measured (32 / 8 heads): 2 x 512 tokens over 4k 78 us (824 TFLOP/s, 49 % of the measured bf16 burst),
-// 2048 tokens over 18k 595 us (982 TFLOP/s, 58 %).  The MMAs alone take 448 us of the latter; the softmax
+// Measured (32 / 8 heads): 2 x 512 tokens over 4k 85 us (757 TFLOP/s, 45 % of the measured bf16 burst),
+// 2048 tokens over 18k 640 us (913 TFLOP/s, 54 %); on the fastest box met 78 and 595, where the steps below
+// were timed.  The MMAs alone take 448 us of the latter; the softmax
 // warps bind it (about 2400 cycles of a tile's 4000 go to the exponentials and their conversion, of
 // which the 128 exponentials themselves need 1024).  Tried: an S region per tile with P written over
 // it 701 us; units of 64 keys with two S regions 734 us; every fourth pair of exponentials as a cubic

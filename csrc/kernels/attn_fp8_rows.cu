@@ -30,10 +30,10 @@
 // however far its scale lies from the others'.  l sums w / vs relative to the share's first vs, so vs may
 // spread over 2^100 in a sequence and head.  m, l, O are fp32.
 //
-// Measured (32 query / 8 KV heads unless said): 256 ragged sequences up to 2304 keys 115 us (5.6 TB/s,
-// 86 % of the measured copy rate; the main kernel alone 106 us), 37 x 3001 with 32 KV heads 83 us (89 %),
-// 7 sequences up to 100k keys with 64 / 8 heads 130 us (88 %), one of 2047 keys 10.3 us (launches and
-// the first loads), 32 x up to 5 tokens over up to 1280 keys 30 us.  With 8 warps an SM instead of 12
+// Measured (32 query / 8 KV heads unless said): 256 ragged sequences up to 2304 keys 117 us (5.5 TB/s,
+// 84 % of the measured copy rate; the main kernel alone 108 us), 37 x 3001 with 32 KV heads 84 us (87 %),
+// 7 sequences up to 100k keys with 64 / 8 heads 132 us (87 %), one of 2047 keys 9.8 us (launches and
+// the first loads), 32 x up to 5 tokens over up to 1280 keys 28 us.  With 8 warps an SM instead of 12
 // the first took 126 us: two warps a scheduler leave it idle most of the time.
 #include <ATen/Functions.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -789,8 +789,8 @@ void fp8_rows(const fp8a::Args& a, bool list, int64_t rows, const CUtensorMap& t
   using namespace fp8d;
   // As many column tiles as hold a decode group (16 columns at a time beyond that), or a list's items,
   // so that one pass over the keys does.  Lists of 64 items over 4000 keys, us with 1 / 2 /
-  // 3 column tiles: 8 rows 94 / 105 / 139, 12 rows 178 / 107 / 140, 20 rows 266 / 192 / 143, 32 rows
-  // 351 / 196 / 257 (two passes of 16 beat 24 + 8).
+  // 3 column tiles: 8 rows 95 / 103 / 132, 12 rows 179 / 104 / 133, 20 rows 268 / 189 / 136, 32 rows
+  // 350 / 193 / 246 (two passes of 16 beat 24 + 8).
   if (list && (rows > 24 || (rows > 8 && rows <= 16))) launch<true, 2>(a, tk, tv, like, st);
   else if (list && rows > 16) launch<true, 3>(a, tk, tv, like, st);
   else if (list) launch<true, 1>(a, tk, tv, like, st);

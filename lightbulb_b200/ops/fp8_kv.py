@@ -202,7 +202,8 @@ def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     ``cu_q`` delimits each sequence's query tokens, the last of its keys, and the work list
     (``tile_seq``, ``tile_row0``: one entry per 256 packed rows, -1 entries skipped) says which
     sequences are computed; with ``causal`` a token sees the keys up to its own.  Rows without a
-    visible key give 0.  ``scale`` defaults to 1 / sqrt(128) (pass 1 / sqrt(true head_dim) for
+    visible key give 0; NaN among a sequence's values reaches its rows that share a tile of keys with
+    it, seen or not.  ``scale`` defaults to 1 / sqrt(128) (pass 1 / sqrt(true head_dim) for
     zero-padded heads).
 
     ``item_rows``: query rows (tokens times ``group``) of the work list's longest item, which decides
