@@ -22,24 +22,24 @@
 //               the sequence's end become zeros.
 //   warps 8-15  softmax, one thread per query row: it reads its row of q once (as f16, scaled by a
 //               power of two and with the softmax scale's sign, into shared memory), then per tile 128
-//               scores from TMEM.  ks of a
-//               16-key slice multiplies its scores, vs goes into the exponent:
+//               scores from TMEM.  ks of a 16-key slice multiplies its scores, vs goes into the exponent:
 //                 P = 2^(s + log2 vs - m' + 7),  m' >= max(s + log2 vs) - 8,
-//               so P is at most 2^15 and keeps f16's 11 bits down to 2^-21 of the largest
-//               contribution; l sums P / vs in fp32.  m' moves only when the maximum passes it by 2^8
-//               (then O is rescaled in TMEM, after the previous tile's P V).
+//               so P is at most 2^15 and keeps f16's 11 bits down to 2^-21 of the largest contribution;
+//               l sums P / vs in fp32 (a scale of 0 stands for a block of zeros: any other does too).  m'
+//               moves only when the maximum passes it by 2^8 (then O is rescaled in TMEM, after the
+//               previous tile's P V).
 // P (f16, in TMEM) is the MMA's A operand; V is read in its key-major layout.  TMEM: O_t at 128 t, S at
 // 256, P_t at 384 + 64 t.  Registers: 512 threads start with 128 each; the softmax warps take 200
 // (40 + 72 + 200 + 200 = 4 * 128 per quarter).  Every wait is bounded; on expiry the kernel records an
 // error and unwinds.
 //
-// Measured (32 / 8 heads): 2 x 512 tokens over 4k 85 us (757 TFLOP/s, 45 % of the measured bf16 burst),
-// 2048 tokens over 18k 640 us (913 TFLOP/s, 54 %); on the fastest box met 78 and 595, where the steps below
-// were timed.  The MMAs alone take 448 us of the latter; the softmax
-// warps bind it (about 2400 cycles of a tile's 4000 go to the exponentials and their conversion, of
-// which the 128 exponentials themselves need 1024).  Tried: an S region per tile with P written over
-// it 701 us; units of 64 keys with two S regions 734 us; every fourth pair of exponentials as a cubic
-// on the FMA pipe 689 us.
+// Measured (32 / 8 heads): 2 x 512 tokens over 4k 86 us (750 TFLOP/s, 44 % of the measured bf16 burst),
+// 2048 tokens over 18k 657 us (889 TFLOP/s, 53 %); on the fastest box met 78 and 595, where the
+// variants below were timed.  The MMAs alone take 448 us of the latter; the softmax warps bind it (about
+// 2400 cycles of a tile's 4000 go to the exponentials and their conversion, of which the 128 exponentials
+// themselves need 1024).  Tried: an S region per tile with P written over it 701 us; units of 64 keys with
+// two S regions 734 us; every fourth pair of exponentials as a cubic on the FMA pipe 689 us.  Where the
+// compiler places the loop moves the time by up to 10 % (634 to 707 us for changes outside it).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 
@@ -372,6 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           ks = a.k_scale[bh];
           vs = a.v_scale[bh];
         }
+        if (vs == 0.f) vs = vs0;     // a block of zeros: any positive scale stands for it
         const float lv = log2f(vs);
         if (j == 0) {
           lv0 = __shfl_sync(0xffffffffu, lv, 0);

@@ -27,8 +27,9 @@
 // 12 (then 13, 14, 15, 8 .. 11): both ldmatrix shapes then touch eight different swizzle rows.
 // Weights are f16 (11 bits) scaled to 2^15 at most, which keeps those bits down to 2^-29 of the
 // largest.  vs is part of a weight's exponent, so a block counts by its softmax weight times its scale,
-// however far its scale lies from the others'.  l sums w / vs relative to the share's first vs, so vs may
-// spread over 2^100 in a sequence and head.  m, l, O are fp32.
+// however far its scale lies from the others'.  l sums w / vs relative to the share's first vs (not scaled
+// by 2^15), so vs may spread over 2^100 in a sequence and head.  A scale of 0 stands for a block of zeros: its
+// keys count in l with the first vs's exponent.  m, l, O are fp32.
 //
 // Measured (32 query / 8 KV heads unless said): 256 ragged sequences up to 2304 keys 117 us (5.5 TB/s,
 // 84 % of the measured copy rate; the main kernel alone 108 us), 37 x 3001 with 32 KV heads 84 us (87 %),
@@ -61,6 +62,7 @@ constexpr int q_smem_of(int nt) { return nt > 2 ? nt * 8 * 32 * 8 : 0; }    // b
 constexpr int MAX_ENTRIES = 4096;
 constexpr int ENTRY_ROWS = 256;               // packed query rows of a work list's item
 constexpr float P_EXP = 15.f;                 // weights are w * 2^15
+constexpr float P_UNIT = 1.f / 32768.f;
 constexpr float VS_SPREAD = 100.f;            // log2 of the largest ratio of V scales that l holds
 
 // A run that starts in a share and goes on in the next ones, for the kernel that joins its parts.
@@ -470,9 +472,10 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
       const int nsl = left > SL ? 2 : 1;
       const float2 sc0 = *reinterpret_cast<const float2*>(s_scale + stage * 4);
       const float2 sc1 = nsl > 1 ? *reinterpret_cast<const float2*>(s_scale + stage * 4 + 2) : sc0;
-      const float lv0 = lg2(sc0.y), lv1 = lg2(sc1.y);
-      if (t == t0) lv_ref = lv0;
-      const float rv0 = ex2(fminf(lv_ref - lv0, VS_SPREAD)), rv1 = ex2(fminf(lv_ref - lv1, VS_SPREAD));
+      if (t == t0) lv_ref = sc0.y > 0.f ? lg2(sc0.y) : sc1.y > 0.f ? lg2(sc1.y) : 0.f;
+      const float lv0 = sc0.y == 0.f ? lv_ref : lg2(sc0.y), lv1 = sc1.y == 0.f ? lv_ref : lg2(sc1.y);
+      const float rv0 = ex2(fminf(lv_ref - lv0, VS_SPREAD) - P_EXP);
+      const float rv1 = ex2(fminf(lv_ref - lv1, VS_SPREAD) - P_EXP);
       // ---- S^T = K Q^T ----
       float s[2][NT][4];
 #pragma unroll
@@ -627,7 +630,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT))
       const float l0 = sum_over_keys(l[n][0]), l1 = sum_over_keys(l[n][1]);
       const int h0 = n * 8 + 2 * t4;
       if (whole) {
-        const float i0 = l0 != 0.f ? 1.f / l0 : 0.f, i1 = l1 != 0.f ? 1.f / l1 : 0.f;
+        const float i0 = l0 != 0.f ? P_UNIT / l0 : 0.f, i1 = l1 != 0.f ? P_UNIT / l1 : 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           if (h0 + j >= co.count) continue;
@@ -727,7 +730,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const Work 
     }
   }
   l = warp_sum(l);
-  const float inv = l != 0.f ? 1.f / l : 0.f, v_ref = ex2(lv_ref);
+  const float inv = l != 0.f ? P_UNIT / l : 0.f, v_ref = ex2(lv_ref);
   const int tok = LIST ? (cut.row + col) / a.group : 0;
   const int head = cut.kvh * a.group + (LIST ? (cut.row + col) % a.group : cut.row + col);
   *reinterpret_cast<uint2*>(a.out + (cut.q0 + tok) * a.out_ld + static_cast<int64_t>(head) * D +

@@ -3,8 +3,8 @@
 The cache is e4m3 ``[num_blocks, Hkv, block_size, 128]`` for K and for V (block size 16, 32 or
 64) with fp32 scales ``[num_blocks, Hkv]``, one per block of tokens and KV head; a stored value
 is ``code * scale``.  :func:`rope_kv_fp8` writes powers of two as scales; the attention takes any
-positive normal ones, V's within a factor of 2**100 in a sequence and head.  One step uses the three
-together::
+positive normal ones, V's within a factor of 2**100 in a sequence and head, and 0 for blocks of
+zeros.  One step uses the three together::
 
     t = ops.step_tables(ctx_lens, q_lens, rows, seq_tables, new_blocks, T, block_size, ...)
     q = ops.rope_kv_fp8(qkv, t.positions, t.slots, cos_sin, k, v, k_scale, v_scale, hq, hkv)

@@ -102,3 +102,41 @@ def test_scores_that_vanish_or_change_sign(dev, form, q_exp, k_exp, scale):
     q = torch.randn(m * 2, 8, D, generator=torch.Generator().manual_seed(3)) * 2.0 ** q_exp
     out, ref, tol = _run(dev, form, (kc, vc, ks, vs, tables), lens, q.bfloat16(), scale)
     assert bool(((out - ref).abs() <= tol).all())
+
+
+@on_devices
+@on_forms
+@pytest.mark.parametrize("blocks", [(0,), (0, 1), (5, 6, 7), (18,), tuple(range(19))])
+def test_scales_of_zero_stand_for_blocks_of_zeros(dev, form, blocks):
+    """A block of zeros may have scales of 0: its values add nothing, its keys count."""
+    lens = [300, 129]
+    kc, vc, ks, vs, tables = _paged_inputs(lens, 2, 16, 13)
+    for b in blocks:
+        for c, s in ((kc, ks), (vc, vs)):
+            c.view(torch.uint8)[tables[0][b]] = 0
+            s[tables[0][b]] = 0
+    m, _ = FORMS[form]
+    q = torch.randn(m * 2, 8, D, generator=torch.Generator().manual_seed(4)).bfloat16()
+    out, ref, tol = _run(dev, form, (kc, vc, ks, vs, tables), lens, q)
+    assert bool(((out - ref).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+@on_forms
+@pytest.mark.parametrize("block", [0, 600, 1249])
+@pytest.mark.parametrize("bits", [0, 115])
+def test_long_sequences_at_both_ends_of_the_spread(form, block, bits):
+    """20,000 keys of equal weight, their V scales 2^-100 of one block's whose keys score ``bits`` less:
+    the sum of the weights over the scales stays in range at both ends."""
+    lens = [20000]
+    kc, vc, ks, vs, tables = _paged_inputs(lens, 1, 16, 17)
+    kc.view(torch.uint8).masked_fill_(kc.view(torch.uint8) != 0x7F, 0)
+    vs[:] = torch.where(torch.isnan(vs), vs, 2.0 ** -90)
+    i = tables[0][block]
+    vs[i], ks[i] = 2.0 ** 10, 1.0
+    kc[i, :, :, 0] = torch.tensor(-bits * math.log(2) * math.sqrt(D) / 16).to(E4M3)
+    m, decode = FORMS[form]
+    q = torch.randn(m, 4, D, generator=torch.Generator().manual_seed(5))
+    q[..., 0] = 16
+    out, ref, tol = _run("cuda", form, (kc, vc, ks, vs, tables), lens, q.bfloat16())
+    assert bool(((out - ref).abs() <= tol).all())
